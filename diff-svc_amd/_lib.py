@@ -90,6 +90,11 @@ class TrainArgs(ctypes.Structure):
                 ("clip_ids", ctypes.c_void_p)]
 
 
+class OrthoCfg(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_int32), ("planes", ctypes.c_int32), ("batch", ctypes.c_int32), ("rows", ctypes.c_int32), ("cols", ctypes.c_int32),
+                ("steps", ctypes.c_int32), ("coef", ctypes.c_float * 3), ("eps", ctypes.c_float), ("scale", ctypes.c_float)]
+
+
 # every symbol include/dsvc.h declares: (name, restype, argtypes)
 _VP = ctypes.c_void_p
 SYMBOLS = [
@@ -154,6 +159,17 @@ SYMBOLS = [
     ("dsvc_trainer_step_end", ctypes.c_int, [_VP, _VP, _VP]),
     ("dsvc_adamw_step", ctypes.c_int, [_VP, _VP, _VP, _VP, ctypes.c_int64, ctypes.c_float, ctypes.c_float, ctypes.c_float, ctypes.c_float,
                                        ctypes.c_float, ctypes.c_int64, _VP, ctypes.c_float, _VP]),
+    ("dsvc_embed_tokens", ctypes.c_int, [_VP, ctypes.c_int32, ctypes.c_int64, _VP, ctypes.c_int64, ctypes.c_int64, ctypes.c_int32, ctypes.c_int32,
+                                         ctypes.c_float, _VP, ctypes.c_int64, _VP, _VP]),
+    ("dsvc_embed_tokens_grad_workspace", ctypes.c_int, [ctypes.c_int64, ctypes.c_int64, ctypes.c_int32, ctypes.POINTER(ctypes.c_int64)]),
+    ("dsvc_embed_tokens_grad", ctypes.c_int, [_VP, ctypes.c_int32, ctypes.c_int64, _VP, ctypes.c_int64, ctypes.c_int32, ctypes.c_int64, ctypes.c_int32,
+                                              ctypes.c_float, ctypes.c_int64, _VP, ctypes.c_int64, ctypes.c_int32, ctypes.c_int32, _VP, ctypes.c_int64, _VP]),
+    ("dsvc_ortho_workspace", ctypes.c_int, [ctypes.POINTER(OrthoCfg), ctypes.POINTER(ctypes.c_int64)]),
+    ("dsvc_orthogonalize", ctypes.c_int, [ctypes.POINTER(OrthoCfg), _VP, ctypes.c_int64, ctypes.c_int64, _VP, ctypes.c_int64, ctypes.c_int64, _VP,
+                                          ctypes.c_int64, _VP]),
+    ("dsvc_muon_step", ctypes.c_int, [ctypes.POINTER(OrthoCfg), _VP, ctypes.c_int64, ctypes.c_int64, _VP, ctypes.c_int64, ctypes.c_int64, _VP, ctypes.c_int64,
+                                      ctypes.c_int64, ctypes.c_float, ctypes.c_float, ctypes.c_int32, ctypes.c_float, _VP, ctypes.c_float, _VP,
+                                      ctypes.c_int64, _VP]),
     ("dsvc_grad_clip_coef", ctypes.c_int, [_VP, ctypes.c_int64, ctypes.c_float, _VP, _VP, _VP]),
 ]
 

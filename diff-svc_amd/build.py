@@ -13,7 +13,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "libdsvc_hip.so")
 OUT_PROF = os.path.join(HERE, "libdsvc_hip_prof.so")
-SOURCES = ["common.hip", "diffnet.hip", "vocoder.hip", "melspec.hip", "train.hip", "hubert.hip", "pe.hip", "cond.hip", "probe.hip"]
+SOURCES = ["common.hip", "diffnet.hip", "vocoder.hip", "melspec.hip", "train.hip", "hubert.hip", "pe.hip", "cond.hip", "embed.hip", "ortho.hip", "probe.hip"]
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-Wall", "-Wno-unused-function",
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",       # no v_pk_{add,mul,fma}_f32: some of their forms give wrong results now and then on gfx950
          "-fvisibility=hidden", "-fvisibility-inlines-hidden",      # the entry points (DSVC_API in include/dsvc.h) are the ONLY dynamic symbols

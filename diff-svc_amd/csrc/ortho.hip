@@ -1,0 +1,584 @@
+// Orthogonalising an update by Newton-Schulz products, and the optimisation step built on it (include/dsvc.h: dsvc_orthogonalize,
+// dsvc_muon_step).
+//
+//   X = G / (||G||_F + eps)      (G transposed if it has more rows than columns, so X is [m x n] with m <= n)
+//   steps times:  A = X X^T,  M = a I + b A + c A A,  X <- M X            (the singular values go through s (a + b s^2 + c s^4))
+//   O = scale * X                (transposed back)
+//
+// Arithmetic: every product is an fp16 MFMA (v_mfma_f32_32x32x16_f16) with fp32 accumulation.  bf16 tensors run on ONE fp16 plane (its 11 bits stay
+// below the 8 of the result: 1.2e-3 against a half step of 1.7e-3 rms); fp32 and fp16 tensors on hi + lo planes and three MFMAs per product
+// (hi hi + hi lo + lo hi: 22 bits per operand, fp32-class, the trainer's own scheme).
+// The planes hold X * 2^12 and A, M * 2^10: |X| and |M| are bounded by the polynomial on [0, 1] (checked on the host for the caller's
+// coefficients), so fp16's top is out of reach and small elements keep their bits; an update whose norm eps swamps is carried with an
+// extra power of two that shrinks as the iterate grows (Scalars::e0).  Norms are summed in fp64: no square of a tiny gradient underflows.
+//
+// Layout: every matrix between the products lies in MFMA FRAGMENT ORDER -- [32-row block][16-wide k step][plane][lane][8]: lane l of a
+// 1 KiB piece holds row l & 31, k = 8 (l >> 5) .. + 7.  A stage of a tile is then a few contiguous KiB that global_load_lds copies into LDS as
+// they lie and ds_read_b128 reads without bank conflicts; the accumulator layout (lane = column, registers = 4 consecutive rows) writes
+// the TRANSPOSED result as whole 512-byte runs, and the untransposed one after the tile went through the matrix core once more against an
+// identity fragment (exact: one fp16 value times one).  Rows and columns are padded with zeros to 128, which every product keeps zero.
+//
+// A and M are symmetric: only the tiles on and above the diagonal are computed, the mirrored tile is written by the same workgroup.
+#include <math.h>
+
+#include "../../include/dsvc.h"
+#include "common.h"
+
+using namespace dsvc;
+
+namespace {
+
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef const half8 __attribute__((address_space(3))) * lds_half8;
+
+constexpr float X_SCALE = 4096.f, A_SCALE = 1024.f;
+constexpr int PAD = 128;                     // rows and columns of every intermediate are padded to this
+constexpr int SUM_BLOCKS = 128;              // partial sums of squares per matrix
+
+enum { F32 = DSVC_DTYPE_F32, F16 = DSVC_DTYPE_F16, BF16 = DSVC_DTYPE_BF16 };
+
+template <int T> struct Elem;
+template <> struct Elem<F32> { typedef float type; };
+template <> struct Elem<F16> { typedef _Float16 type; };
+template <> struct Elem<BF16> { typedef __bf16 type; };
+
+struct View { long long ld, bs; };           // elements between rows / between matrices
+
+// per matrix, written by the normalising kernel's block 0 and read by the products
+struct Scalars { int e0; };
+
+struct MuonArgs {                            // momentum: null for the plain operator
+    float* mom; View mv;
+    float mu, lr, wd;
+    int nesterov;
+    const float* gscale_dev;
+    float gscale;
+};
+
+// u = the tensor that is orthogonalised, from the gradient and the UPDATED momentum
+__device__ __forceinline__ float muon_mom(const MuonArgs& u, float g, float m) { return fmaf(u.mu, m, (1.f - u.mu) * g); }
+__device__ __forceinline__ float muon_u(const MuonArgs& u, float g, float m) { return u.nesterov ? fmaf(u.mu, m, (1.f - u.mu) * g) : m; }
+
+// ---- sums of squares (fp64), and the momentum update on the way: grid (blocks, matrices).  Partials are combined in a fixed order. ----
+template <int T, bool MUON>
+__global__ __launch_bounds__(256) void k_ns_sums(const void* __restrict__ in, View iv, int rows, int cols, MuonArgs mu, double* __restrict__ part,
+                                                 int* __restrict__ count, int n_count) {
+    typedef typename Elem<T>::type E;
+    const int b = blockIdx.y;
+    const E* src = (const E*)in + b * iv.bs;
+    float* mom = MUON ? mu.mom + b * mu.mv.bs : nullptr;
+    const float gs = MUON ? (mu.gscale_dev ? *mu.gscale_dev : mu.gscale) : 1.f;
+    for (int i = (blockIdx.y * gridDim.x + blockIdx.x) * 256 + threadIdx.x; i < n_count; i += gridDim.x * gridDim.y * 256) count[i] = 0;
+    const long long n = (long long)rows * cols;
+    double s = 0.0;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
+        const int r = (int)(i / cols), c = (int)(i - (long long)r * cols);
+        float v = (float)src[r * iv.ld + c];
+        if (MUON) {
+            const float g = v * gs;
+            float* p = mom + r * mu.mv.ld + c;
+            const float m = muon_mom(mu, g, *p);
+            *p = m;
+            v = muon_u(mu, g, m);
+        }
+        s += (double)v * (double)v;
+    }
+    __shared__ double red[256];
+    red[threadIdx.x] = s;
+    __syncthreads();
+    for (int k = 128; k > 0; k >>= 1) {
+        if ((int)threadIdx.x < k) red[threadIdx.x] += red[threadIdx.x + k];
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) part[(long long)b * gridDim.x + blockIdx.x] = red[0];
+}
+
+// ---- normalise and lay out: one workgroup = a 64 x 64 tile of X, written in fragment order as X (k = columns) and X^T (k = rows) ----
+template <int T, bool MUON, int P>
+__global__ __launch_bounds__(256) void k_ns_prep(const void* __restrict__ in, View iv, int rows, int cols, int tall, MuonArgs mu, const double* __restrict__ part,
+                                                 int n_part, double eps, _Float16* __restrict__ x, _Float16* __restrict__ xt, int mp, int np, Scalars* __restrict__ sc) {
+    typedef typename Elem<T>::type E;
+    const int b = blockIdx.z, i0 = blockIdx.y * 64, j0 = blockIdx.x * 64, tid = threadIdx.x;
+    __shared__ double red[128];
+    __shared__ float tile[64][65];
+    if (tid < 128) red[tid] = tid < n_part ? part[(long long)b * n_part + tid] : 0.0;
+    __syncthreads();
+    for (int k = 64; k > 0; k >>= 1) {
+        if (tid < k) red[tid] += red[tid + k];
+        __syncthreads();
+    }
+    const double norm = sqrt(red[0]), t = norm / (norm + eps);
+    // t < 1/2 only where eps matters: planes carry 2^e0 more
+    int e0 = 0;
+    if (t < 0.5) e0 = t > 1e-18 ? -ilogb(t) - 1 : 59;
+    if (blockIdx.x == 0 && blockIdx.y == 0 && tid == 0) sc[b].e0 = e0;
+    const double f = ldexp((double)X_SCALE, e0) / (norm + eps);
+    const E* src = (const E*)in + b * iv.bs;
+    const float* mom = MUON ? mu.mom + b * mu.mv.bs : nullptr;
+    const float gs = MUON ? (mu.gscale_dev ? *mu.gscale_dev : mu.gscale) : 1.f;
+    const int r0 = tall ? j0 : i0, c0 = tall ? i0 : j0;
+    for (int k = tid; k < 4096; k += 256) {
+        const int r = k >> 6, c = k & 63;
+        float v = 0.f;
+        if (r0 + r < rows && c0 + c < cols) {
+            v = (float)src[(long long)(r0 + r) * iv.ld + c0 + c];
+            if (MUON) v = muon_u(mu, v * gs, mom[(long long)(r0 + r) * mu.mv.ld + c0 + c]);
+            v = (float)((double)v * f);
+        }
+        if (tall) tile[c][r] = v; else tile[r][c] = v;          // tile[i][j]
+    }
+    __syncthreads();
+    const int wave = tid >> 6, lane = tid & 63;
+    const int nk_x = np >> 4, nk_t = mp >> 4;
+    _Float16* xb = x + (long long)b * mp * np * P;
+    _Float16* tb = xt + (long long)b * mp * np * P;
+    for (int q = wave; q < 16; q += 4) {                        // 8 pieces of X, 8 of X^T
+        const int blk = (q >> 2) & 1, k16 = q & 3, row = 32 * blk + (lane & 31), k = 16 * k16 + 8 * (lane >> 5);
+        half8 hi, lo;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float v = q < 8 ? tile[row][k + e] : tile[k + e][row];
+            hi[e] = (_Float16)v;
+            lo[e] = (_Float16)(v - (float)hi[e]);
+        }
+        _Float16* d = q < 8 ? xb + (((long long)((i0 >> 5) + blk) * nk_x + (j0 >> 4) + k16) * P) * 512
+                            : tb + (((long long)((j0 >> 5) + blk) * nk_t + (i0 >> 4) + k16) * P) * 512;
+        *(half8*)(d + lane * 8) = hi;
+        if (P == 2) *(half8*)(d + 512 + lane * 8) = lo;
+    }
+}
+
+// ---- the products ----------------------------------------------------------------------------------------------------------------------
+enum { GRAM, POLY, FULL, FINAL };
+
+struct NsGemm {
+    const _Float16 *a, *b;                   // fragment-order operands, rows x K each: result[i][j] = sum_k a[i][k] b[j][k]
+    long long a_bs, b_bs;                    // halfs per matrix
+    int nk16;                                // K / 16
+    int tiles_i, tiles_j, n_tiles, batch, slices;
+    float* part; int* count;                 // split K: partial tiles and arrival counters
+    _Float16 *o, *ot;                        // FULL: result (k = j), transposed result (k = i); GRAM / POLY: ot only (symmetric)
+    long long o_bs, ot_bs;
+    int o_nk16, ot_nk16;
+    const _Float16* am;                      // POLY: A
+    float c0, c1, c2;                        // POLY: c0 on the diagonal, c1 A, c2 acc; others: c2 acc
+    const Scalars* sc;
+    int step, dec;                           // e_k = max(0, e0 - k dec)
+    // FINAL
+    void* out; View ov;
+    int dtype, m, n, tall;
+    MuonArgs mu;                             // mu.mom: out is the parameter, out <- (1 - lr wd) out - lr result
+};
+
+template <int N> __device__ __forceinline__ void wait_vm_lgkm() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory"); }
+
+// 32 x 32 accumulator tile whose lane is the ROW of the stored matrix: rows 32 rowblk .. + 31, k = 16 k16 .. + 31
+template <int P>
+__device__ __forceinline__ void store_frag(_Float16* __restrict__ base, int nk16, int rowblk, int k16, int lane, const half4 (&hi)[4], const half4 (&lo)[4]) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        _Float16* d = base + ((long long)rowblk * nk16 + k16 + (q >> 1)) * P * 512 + ((lane & 31) + 32 * (q & 1)) * 8 + 4 * (lane >> 5);
+        *(half4*)d = hi[q];
+        if (P == 2) *(half4*)(d + 512) = lo[q];
+    }
+}
+
+// lane / register roles of a tile exchanged: t[c][r] of v[r][c], exact
+__device__ __forceinline__ void transpose_tile(const half4 (&v)[4], const half8 (&ident)[2], half4 (&t)[4]) {
+    f32x16 acc;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[r] = 0.f;
+#pragma unroll
+    for (int pi = 0; pi < 2; ++pi) {
+        const half8 a = __builtin_shufflevector(v[2 * pi], v[2 * pi + 1], 0, 1, 2, 3, 4, 5, 6, 7);
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ident[pi], acc, 0, 0, 0);
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) t[r >> 2][r & 3] = (_Float16)acc[r];
+}
+
+// One workgroup = a tile of (32 TM WR) x (32 TN WC) of one matrix (or one K slice of it); WR x WC waves of TM x TN accumulator tiles; NST stages of
+// KS k steps in LDS.
+template <int P, int TM, int TN, int WR, int WC, int KS, int NST, int MODE>
+__global__ __launch_bounds__(WR * WC * 64) void k_ns_gemm(const NsGemm g) {
+    constexpr int NW = WR * WC, RA = TM * WR, RB = TN * WC, U = KS * P, PIECES = (RA + RB) * U, PER = PIECES / NW;
+    constexpr bool SYM = MODE == GRAM || MODE == POLY;
+    static_assert(PIECES % NW == 0 && PER * (NST - 2) < 64, "");
+    extern __shared__ __attribute__((aligned(1024))) char smem[];
+    // workgroups of one XCD (id % 8) take neighbouring tiles: they share operand rows in its L2
+    const int total = g.batch * g.n_tiles * g.slices, per = (total + 7) / 8;
+    const int lin = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if ((int)(blockIdx.x >> 3) >= per || lin >= total) return;
+    const int tile = lin % g.n_tiles, bs = lin / g.n_tiles, slice = bs % g.slices, b = bs / g.slices;
+    int ti, tj;
+    if (SYM) {
+        tj = (int)((sqrtf(8.f * tile + 1.f) - 1.f) * 0.5f);
+        while ((tj + 1) * (tj + 2) / 2 <= tile) ++tj;
+        while (tj * (tj + 1) / 2 > tile) --tj;
+        ti = tile - tj * (tj + 1) / 2;
+    } else {
+        tj = tile / g.tiles_i;
+        ti = tile - tj * g.tiles_i;
+    }
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int wr = wave / WC, wc = wave % WC;
+    const int n_stages_all = g.nk16 / KS, ps = (n_stages_all + g.slices - 1) / g.slices;
+    const int s_begin = slice * ps, n_stages = min(n_stages_all - s_begin, ps);     // (<= 0 for a slice behind the end: contributes zeros)
+    const _Float16* abase = g.a + b * g.a_bs + (long long)ti * RA * g.nk16 * P * 512;
+    const _Float16* bbase = g.b + b * g.b_bs + (long long)tj * RB * g.nk16 * P * 512;
+    const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) char*)smem;
+
+    auto dma = [&](int s) {
+        char* dst = smem + (s % NST) * (PIECES * 1024);
+        const long long k = (long long)(s_begin + s) * U;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int pc = wave + NW * i, rb = pc / U, u = pc % U;
+            const _Float16* src = (rb < RA ? abase + (long long)rb * g.nk16 * (P * 512) : bbase + (long long)(rb - RA) * g.nk16 * (P * 512)) + (k + u) * 512 + lane * 8;
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src, (__attribute__((address_space(3))) void*)(dst + pc * 1024), 16, 0, 0);
+        }
+    };
+
+    f32x16 acc[TM][TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+
+#pragma unroll
+    for (int s = 0; s < NST - 1; ++s)
+        if (s < n_stages) dma(s);
+    for (int s = 0; s < n_stages; ++s) {
+        // this wave's copies of stage s have landed (vmcnt retires in order) and its own LDS reads of stage s - 1 are done; behind the barrier
+        // that holds for every wave, so buffer (s + NST - 1) % NST = (s - 1) % NST may be overwritten
+        if (s + NST - 2 < n_stages) wait_vm_lgkm<PER * (NST - 2)>();
+        else wait_vm_lgkm<0>();
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (s + NST - 1 < n_stages) dma(s + NST - 1);
+        const unsigned buf = lds0 + (unsigned)(s % NST) * (PIECES * 1024) + (unsigned)lane * 16u;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            half8 fa[TM][P], fb[TN][P];
+#pragma unroll
+            for (int p = 0; p < P; ++p) {
+#pragma unroll
+                for (int i = 0; i < TM; ++i) fa[i][p] = *(lds_half8)(size_t)(buf + (unsigned)(((wr * TM + i) * U + k * P + p) * 1024));
+#pragma unroll
+                for (int j = 0; j < TN; ++j) fb[j][p] = *(lds_half8)(size_t)(buf + (unsigned)(((RA + wc * TN + j) * U + k * P + p) * 1024));
+            }
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j) {
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[i][0], fb[j][0], acc[i][j], 0, 0, 0);
+                    if constexpr (P == 2) {
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[i][1], fb[j][0], acc[i][j], 0, 0, 0);
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[i][0], fb[j][1], acc[i][j], 0, 0, 0);
+                    }
+                }
+        }
+    }
+
+    if (g.slices > 1) {
+        // every slice leaves its partial tile; the workgroup that arrives last adds them up in slice order (whoever it is: the same sum)
+        const int slot = (b * g.n_tiles + tile);
+        f32x4* mine = (f32x4*)g.part + ((long long)slot * g.slices + slice) * (TM * TN * 4 * NW * 64) + threadIdx.x;
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    mine[((i * TN + j) * 4 + q) * (NW * 64)] = f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+        __threadfence();
+        __syncthreads();
+        int* last = (int*)smem;
+        if (threadIdx.x == 0) {
+            const int at = atomicAdd(g.count + slot, 1);
+            *last = at == g.slices - 1;
+            if (at == g.slices - 1) g.count[slot] = 0;           // for the next launch
+        }
+        __syncthreads();
+        if (!*last) return;
+        __threadfence();
+        const f32x4* all = (const f32x4*)g.part + (long long)slot * g.slices * (TM * TN * 4 * NW * 64) + threadIdx.x;
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    f32x4 v = all[((i * TN + j) * 4 + q) * (NW * 64)];
+                    for (int z = 1; z < g.slices; ++z) v += all[(long long)z * (TM * TN * 4 * NW * 64) + ((i * TN + j) * 4 + q) * (NW * 64)];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[i][j][4 * q + e] = v[e];
+                }
+    }
+
+    // ---- epilogue: register r of a lane = row 8 (r >> 2) + 4 (lane >> 5) + (r & 3), column lane & 31 ----
+    const int e0 = g.sc[b].e0, ek = max(0, e0 - g.step * g.dec), ek1 = max(0, e0 - (g.step + 1) * g.dec);
+    float c2 = g.c2;
+    if (MODE == GRAM) c2 = ldexpf(c2, -2 * ek);
+    if (MODE == FULL) c2 = ldexpf(c2, ek1 - ek);
+    if (MODE == FINAL) c2 = ldexpf(c2, -ek);
+    half8 ident[2];
+#pragma unroll
+    for (int pi = 0; pi < 2; ++pi)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ident[pi][e] = (lane & 31) == 16 * pi + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3) ? (_Float16)1.f : (_Float16)0.f;
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+            const int bi = ti * RA + wr * TM + i, bj = tj * RB + wc * TN + j;      // 32-blocks of the result
+            if constexpr (MODE == FINAL) {
+                const int col = 32 * bj + (lane & 31);
+                if (col >= g.n) continue;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int row = 32 * bi + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
+                    if (row >= g.m) continue;
+                    const long long at = b * g.ov.bs + (g.tall ? col * g.ov.ld + row : row * g.ov.ld + col);
+                    float v = acc[i][j][r] * c2;
+                    if (g.mu.mom) {
+                        const float p = g.dtype == F32 ? ((float*)g.out)[at] : g.dtype == F16 ? (float)((_Float16*)g.out)[at] : (float)((__bf16*)g.out)[at];
+                        v = fmaf(-g.mu.lr, v, (1.f - g.mu.lr * g.mu.wd) * p);
+                    }
+                    if (g.dtype == F32) ((float*)g.out)[at] = v;
+                    else if (g.dtype == F16) ((_Float16*)g.out)[at] = (_Float16)v;
+                    else ((__bf16*)g.out)[at] = (__bf16)v;
+                }
+            } else {
+                half4 am_hi[4], am_lo[4];
+                if constexpr (MODE == POLY) {
+                    const _Float16* am = g.am + b * g.ot_bs;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const _Float16* s = am + ((long long)bj * g.ot_nk16 + 2 * bi + (q >> 1)) * P * 512 + ((lane & 31) + 32 * (q & 1)) * 8 + 4 * (lane >> 5);
+                        am_hi[q] = *(const half4*)s;
+                        if (P == 2) am_lo[q] = *(const half4*)(s + 512);
+                    }
+                }
+                half4 hi[4], lo[4];
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    float v = acc[i][j][r] * c2;
+                    if constexpr (MODE == POLY) {
+                        float am = (float)am_hi[r >> 2][r & 3];
+                        if (P == 2) am += (float)am_lo[r >> 2][r & 3];
+                        v = fmaf(g.c1, am, v);
+                        if (bi == bj && 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3) == (lane & 31)) v += g.c0;
+                    }
+                    hi[r >> 2][r & 3] = (_Float16)v;
+                    if (P == 2) lo[r >> 2][r & 3] = (_Float16)(v - (float)hi[r >> 2][r & 3]);
+                }
+                store_frag<P>(g.ot + b * g.ot_bs, g.ot_nk16, bj, 2 * bi, lane, hi, lo);
+                if (MODE == FULL || ti != tj) {
+                    half4 th[4], tl[4];
+                    transpose_tile(hi, ident, th);
+                    if (P == 2) transpose_tile(lo, ident, tl);
+                    if (MODE == FULL) store_frag<P>(g.o + b * g.o_bs, g.o_nk16, bi, 2 * bj, lane, th, tl);
+                    else store_frag<P>(g.ot + b * g.ot_bs, g.ot_nk16, bi, 2 * bj, lane, th, tl);
+                }
+            }
+        }
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------------------------------
+template <int P, int MODE>
+int gemm(NsGemm& g, int mi, int nj, hipStream_t st) {
+    constexpr int TM = 2, TN = 2, WR = 2, WC = 2, KS = 4 / P, NST = 2;
+    constexpr int LDS = (TM * WR + TN * WC) * KS * P * 1024 * NST;
+    g.tiles_i = mi / (32 * TM * WR);
+    g.tiles_j = nj / (32 * TN * WC);
+    g.n_tiles = MODE == GRAM || MODE == POLY ? g.tiles_i * (g.tiles_i + 1) / 2 : g.tiles_i * g.tiles_j;
+    auto kernel = k_ns_gemm<P, TM, TN, WR, WC, KS, NST, MODE>;
+    const long long total = (long long)g.batch * g.n_tiles * g.slices;
+    if (total >= (1LL << 24)) return fail(DSVC_EINVAL, "orthogonalize: %lld tiles", total);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((total + 7) / 8 * 8)), dim3(WR * WC * 64), LDS, st, g);
+    DSVC_HIP(hipGetLastError());
+    return DSVC_OK;
+}
+
+struct Plan {
+    int P, m, n, mp, np, tall, n_part, dec;
+    long long off_part, off_sc, off_count, n_count, off_x, off_xt[2], off_a, off_m, bytes;
+};
+
+// The largest singular value that the polynomial can reach from [0, 1] and the largest |a + b s^2 + c s^4| on the way: both stay far from where the
+// fp16 planes end (65504 / X_SCALE, 65504 / A_SCALE).
+int check_coefficients(const float* c, int steps, double* growth) {
+    double s_max = 1.0, most = 0.0;
+    for (int k = 0; k < 3; ++k)
+        if (!isfinite(c[k])) return fail(DSVC_EINVAL, "orthogonalize: coefficient %d is not finite", k);
+    for (int k = 0; k < steps; ++k) {
+        double next = 0.0;
+        for (int i = 0; i <= 4096; ++i) {
+            const double s = s_max * i / 4096, l = s * s, f = c[0] + l * (c[1] + l * c[2]);
+            if (fabs(f) > most) most = fabs(f);
+            if (fabs(f * s) > next) next = fabs(f * s);
+        }
+        s_max = 1.01 * next;
+        if (s_max * s_max > 48.0 || most > 48.0 || s_max > 12.0)
+            return fail(DSVC_EINVAL, "orthogonalize: the coefficients (%g, %g, %g) take singular values from [0, 1] to %g", c[0], c[1], c[2], s_max);
+        if (s_max < 1.0) s_max = 1.0;
+    }
+    *growth = most;
+    return DSVC_OK;
+}
+
+int make_plan(const dsvc_ortho_cfg* c, Plan* p) {
+    if (!c) return fail(DSVC_EINVAL, "null argument");
+    if (c->dtype < F32 || c->dtype > BF16) return fail(DSVC_EINVAL, "orthogonalize: unknown type %d", c->dtype);
+    if (c->planes != 0 && c->planes != 1 && c->planes != 2) return fail(DSVC_EINVAL, "orthogonalize: %d planes (1, 2 or 0: by type)", c->planes);
+    if (c->batch < 0 || c->rows < 0 || c->cols < 0) return fail(DSVC_EINVAL, "orthogonalize: bad shape [%d, %d, %d]", c->batch, c->rows, c->cols);
+    if (c->rows > (1 << 20) || c->cols > (1 << 20) || c->batch > 65535) return fail(DSVC_EINVAL, "orthogonalize: shape [%d, %d, %d] is too large", c->batch, c->rows, c->cols);
+    if (c->steps < 1 || c->steps > 64) return fail(DSVC_EINVAL, "orthogonalize: %d steps", c->steps);
+    if (!(c->eps >= 0.f) || !isfinite(c->eps)) return fail(DSVC_EINVAL, "orthogonalize: eps %g", c->eps);
+    if (!isfinite(c->scale)) return fail(DSVC_EINVAL, "orthogonalize: scale %g", c->scale);
+    double growth = 0.0;
+    DSVC_TRY(check_coefficients(c->coef, c->steps, &growth));
+    *p = Plan{};
+    p->dec = growth > 1.0 ? (int)ceil(log2(growth) + 1e-6) : 0;
+    p->P = c->planes ? c->planes : c->dtype == BF16 ? 1 : 2;
+    p->tall = c->rows > c->cols;
+    p->m = p->tall ? c->cols : c->rows;
+    p->n = p->tall ? c->rows : c->cols;
+    if (!c->batch || !p->m) return DSVC_OK;
+    p->mp = round_up(p->m, PAD);
+    p->np = round_up(p->n, PAD);
+    const long long want = ((long long)p->m * p->n + 4095) / 4096;
+    p->n_part = (int)(want < SUM_BLOCKS ? want : SUM_BLOCKS);
+    long long at = 0;
+    auto take = [&](long long bytes) { const long long o = at; at += (bytes + 1023) / 1024 * 1024; return o; };
+    const long long B = c->batch, xs = B * p->mp * p->np * p->P * 2, as = B * p->mp * p->mp * p->P * 2;
+    p->off_part = take(B * p->n_part * 8);
+    p->off_sc = take(B * (long long)sizeof(Scalars));
+    p->n_count = 0;
+    p->off_count = take(p->n_count * 4);
+    p->off_x = take(xs);
+    p->off_xt[0] = take(xs);
+    p->off_xt[1] = take(xs);
+    p->off_a = take(as);
+    p->off_m = take(as);
+    p->bytes = at;
+    return DSVC_OK;
+}
+
+template <int T, bool MUON, int P>
+int prep(const dsvc_ortho_cfg* c, const Plan& p, const void* in, View iv, const MuonArgs& mu, char* ws, hipStream_t st) {
+    hipLaunchKernelGGL((k_ns_sums<T, MUON>), dim3(p.n_part, c->batch), dim3(256), 0, st, in, iv, c->rows, c->cols, mu, (double*)(ws + p.off_part),
+                       (int*)(ws + p.off_count), (int)p.n_count);
+    hipLaunchKernelGGL((k_ns_prep<T, MUON, P>), dim3(p.np / 64, p.mp / 64, c->batch), dim3(256), 0, st, in, iv, c->rows, c->cols, p.tall, mu,
+                       (const double*)(ws + p.off_part), p.n_part, (double)c->eps, (_Float16*)(ws + p.off_x), (_Float16*)(ws + p.off_xt[0]), p.mp, p.np,
+                       (Scalars*)(ws + p.off_sc));
+    DSVC_HIP(hipGetLastError());
+    return DSVC_OK;
+}
+
+template <bool MUON, int P>
+int prep_t(const dsvc_ortho_cfg* c, const Plan& p, const void* in, View iv, const MuonArgs& mu, char* ws, hipStream_t st) {
+    if (c->dtype == F32) return prep<F32, MUON, P>(c, p, in, iv, mu, ws, st);
+    if (c->dtype == F16) return prep<F16, MUON, P>(c, p, in, iv, mu, ws, st);
+    return prep<BF16, MUON, P>(c, p, in, iv, mu, ws, st);
+}
+
+template <int P>
+int iterate(const dsvc_ortho_cfg* c, const Plan& p, void* out, View ov, const MuonArgs& mu, char* ws, hipStream_t st) {
+    const long long xs = (long long)p.mp * p.np * P, as = (long long)p.mp * p.mp * P;
+    _Float16 *x = (_Float16*)(ws + p.off_x), *a = (_Float16*)(ws + p.off_a), *m = (_Float16*)(ws + p.off_m);
+    for (int k = 0; k < c->steps; ++k) {
+        _Float16 *xt = (_Float16*)(ws + p.off_xt[k & 1]), *xt1 = (_Float16*)(ws + p.off_xt[(k + 1) & 1]);
+        NsGemm g{};
+        g.batch = c->batch; g.slices = 1; g.sc = (const Scalars*)(ws + p.off_sc); g.step = k; g.dec = p.dec;
+        g.a = g.b = x; g.a_bs = g.b_bs = xs; g.nk16 = p.np / 16;
+        g.ot = a; g.ot_bs = as; g.ot_nk16 = p.mp / 16;
+        g.c2 = A_SCALE / (X_SCALE * X_SCALE);
+        DSVC_TRY((gemm<P, GRAM>(g, p.mp, p.mp, st)));
+        g.a = g.b = a; g.a_bs = g.b_bs = as; g.nk16 = p.mp / 16;
+        g.ot = m; g.am = a;
+        g.c0 = c->coef[0] * A_SCALE; g.c1 = c->coef[1]; g.c2 = c->coef[2] / A_SCALE;
+        DSVC_TRY((gemm<P, POLY>(g, p.mp, p.mp, st)));
+        g.a = m; g.b = xt; g.b_bs = xs;
+        g.o = x; g.o_bs = xs; g.o_nk16 = p.np / 16;
+        g.ot = xt1; g.ot_bs = xs;
+        g.c2 = 1.f / A_SCALE;
+        if (k + 1 < c->steps) { DSVC_TRY((gemm<P, FULL>(g, p.mp, p.np, st))); continue; }
+        g.c2 = c->scale / (A_SCALE * X_SCALE);
+        g.out = out; g.ov = ov; g.dtype = c->dtype; g.m = p.m; g.n = p.n; g.tall = p.tall; g.mu = mu;
+        DSVC_TRY((gemm<P, FINAL>(g, p.mp, p.np, st)));
+    }
+    return DSVC_OK;
+}
+
+int check_view(const char* what, int64_t ld, int64_t bs, int rows, int cols, int batch, bool written) {
+    if (ld < cols && rows > 1) return fail(DSVC_EINVAL, "orthogonalize: %s: row stride %lld < %d columns", what, (long long)ld, cols);
+    if (ld < 0 || bs < 0) return fail(DSVC_EINVAL, "orthogonalize: %s: negative stride", what);
+    if (written && batch > 1 && bs < (int64_t)(rows - 1) * ld + cols) return fail(DSVC_EINVAL, "orthogonalize: %s: matrices overlap (stride %lld)", what, (long long)bs);
+    return DSVC_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int dsvc_ortho_workspace(const dsvc_ortho_cfg* c, int64_t* bytes) {
+    if (!bytes) return fail(DSVC_EINVAL, "null argument");
+    Plan p;
+    DSVC_TRY(make_plan(c, &p));
+    *bytes = p.bytes;
+    return DSVC_OK;
+}
+
+int dsvc_orthogonalize(const dsvc_ortho_cfg* c, const void* in, int64_t in_ld, int64_t in_bs, void* out, int64_t out_ld, int64_t out_bs, void* workspace,
+                       int64_t workspace_bytes, void* stream) {
+    Plan p;
+    DSVC_TRY(make_plan(c, &p));
+    if (!c->batch || !p.m) return DSVC_OK;
+    if (!in || !out || !workspace) return fail(DSVC_EINVAL, "null argument");
+    if (workspace_bytes < p.bytes || (uintptr_t)workspace % 256) return fail(DSVC_EINVAL, "orthogonalize: workspace of %lld bytes at %p, need %lld on 256", (long long)workspace_bytes, workspace, p.bytes);
+    DSVC_TRY(check_view("input", in_ld, in_bs, c->rows, c->cols, c->batch, false));
+    DSVC_TRY(check_view("output", out_ld, out_bs, c->rows, c->cols, c->batch, true));
+    char* ws = (char*)workspace;
+    hipStream_t st = (hipStream_t)stream;
+    const MuonArgs none{};
+    const View iv{in_ld, in_bs}, ov{out_ld, out_bs};
+    if (p.P == 2) {
+        DSVC_TRY((prep_t<false, 2>(c, p, in, iv, none, ws, st)));
+        return iterate<2>(c, p, out, ov, none, ws, st);
+    }
+    DSVC_TRY((prep_t<false, 1>(c, p, in, iv, none, ws, st)));
+    return iterate<1>(c, p, out, ov, none, ws, st);
+}
+
+int dsvc_muon_step(const dsvc_ortho_cfg* c, void* param, int64_t param_ld, int64_t param_bs, const void* grad, int64_t grad_ld, int64_t grad_bs, float* momentum,
+                   int64_t mom_ld, int64_t mom_bs, float lr, float mu, int32_t nesterov, float weight_decay, const float* grad_scale_dev, float grad_scale,
+                   void* workspace, int64_t workspace_bytes, void* stream) {
+    Plan p;
+    DSVC_TRY(make_plan(c, &p));
+    if (!isfinite(lr) || !isfinite(weight_decay) || !(mu >= 0.f && mu < 1.f)) return fail(DSVC_EINVAL, "muon_step: lr %g, weight decay %g, momentum %g", lr, weight_decay, mu);
+    if (!c->batch || !p.m) return DSVC_OK;
+    if (!param || !grad || !momentum || !workspace) return fail(DSVC_EINVAL, "null argument");
+    if (workspace_bytes < p.bytes || (uintptr_t)workspace % 256) return fail(DSVC_EINVAL, "muon_step: workspace of %lld bytes at %p, need %lld on 256", (long long)workspace_bytes, workspace, p.bytes);
+    DSVC_TRY(check_view("parameter", param_ld, param_bs, c->rows, c->cols, c->batch, true));
+    DSVC_TRY(check_view("gradient", grad_ld, grad_bs, c->rows, c->cols, c->batch, false));
+    DSVC_TRY(check_view("momentum", mom_ld, mom_bs, c->rows, c->cols, c->batch, true));
+    char* ws = (char*)workspace;
+    hipStream_t st = (hipStream_t)stream;
+    const MuonArgs u{momentum, View{mom_ld, mom_bs}, mu, lr, weight_decay, nesterov, grad_scale_dev, grad_scale};
+    const View gv{grad_ld, grad_bs}, pv{param_ld, param_bs};
+    if (p.P == 2) {
+        DSVC_TRY((prep_t<true, 2>(c, p, grad, gv, u, ws, st)));
+        return iterate<2>(c, p, param, pv, u, ws, st);
+    }
+    DSVC_TRY((prep_t<true, 1>(c, p, grad, gv, u, ws, st)));
+    return iterate<1>(c, p, param, pv, u, ws, st);
+}
+
+}  // extern "C"

@@ -1,0 +1,117 @@
+"""Orthogonalised updates of matrix parameters (csrc/ortho.hip): the Newton-Schulz iteration and the optimisation step built on it.
+
+  X = G / (||G||_F + eps);  steps times:  A = X X^T,  X <- (a I + b A + c A A) X;  O = scale * X
+
+takes every singular value s of the normalised update through s (a + b s^2 + c s^4): with the default coefficients all of them end between about
+0.7 and 1.2, so O is close to U V^T of G = U S V^T.  ``muon_step_`` orthogonalises the (Nesterov) momentum of a gradient and takes the weight step.
+
+Types: float32 and float16 tensors run on split fp16 operands (``precision="f16_x3"``: fp32-class, three matrix-core products per product), bfloat16
+ones on single fp16 operands (``"f16"``); either can be asked for.  Accumulation, norms and momentum are float32 or wider."""
+import ctypes
+import math
+
+import torch
+
+from . import _lib
+from ._lib import check, lib
+from .tokens import DTYPES, on_device
+
+COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+PLANES = {None: 0, "f16": 1, "f16_x3": 2}
+
+
+def rms_scale(rows, cols, rms=0.2):
+    """The scale at which an orthogonalised [rows, cols] update has elements of root mean square ``rms``: 0.2 is about an AdamW step's, so that one
+    learning rate serves both."""
+    return rms * math.sqrt(max(rows, cols))
+
+
+def _cfg(t, steps, coefficients, eps, scale, precision):
+    if precision not in PLANES:
+        raise ValueError("precision must be one of %s, got %r" % ([k for k in PLANES if k], precision))
+    if len(coefficients) != 3:
+        raise ValueError("three coefficients, got %r" % (coefficients,))
+    B, m, n = t.shape
+    return _lib.OrthoCfg(DTYPES[t.dtype], PLANES[precision], B, m, n, steps, (ctypes.c_float * 3)(*coefficients), eps, scale)
+
+
+def _check(name, t):
+    if t.dtype not in DTYPES:
+        raise TypeError("diffsvc_amd: %s must be float32, float16 or bfloat16, got %s" % (name, t.dtype))
+    if t.dim() < 2:
+        raise ValueError("%s must be a matrix or a batch of matrices, got shape %s" % (name, tuple(t.shape)))
+    if not t.is_cuda:
+        raise RuntimeError("diffsvc_amd: %s must live on the HIP device; there is no CPU path" % name)
+
+
+def _matrices(name, t, copy):
+    """t as [batch, rows, columns] with unit stride along the rows; ``copy``: in a new tensor where it does not lie so, else refused."""
+    m, n = t.shape[-2:]
+    if t.dim() == 2:
+        v = t.unsqueeze(0)
+    elif t.dim() == 3:
+        v = t
+    else:
+        v = t.reshape(-1, m, n) if copy else t.view(-1, m, n)
+    ld, bs = v.stride(1), v.stride(0)
+    if (n <= 1 or v.stride(2) == 1) and (m <= 1 or ld >= n) and (v.shape[0] <= 1 or bs >= (m - 1) * ld + n):
+        return v
+    if copy:
+        return v.contiguous()
+    raise ValueError("%s is written in place: it needs rows of unit stride and matrices that do not overlap, got strides %s" % (name, t.stride()))
+
+
+def _workspace(cfg, device):
+    need = ctypes.c_int64(0)
+    check(lib().dsvc_ortho_workspace(ctypes.byref(cfg), ctypes.byref(need)))
+    return torch.empty(need.value, device=device, dtype=torch.uint8)
+
+
+@torch.no_grad()
+def orthogonalize(x, steps=5, coefficients=COEFFICIENTS, eps=1e-7, scale=1.0, precision=None, out=None):
+    """scale * the Newton-Schulz iterate of every matrix of x [..., rows, cols], in x's type.  ``out`` may be x itself."""
+    _check("x", x)
+    v = _matrices("x", x, True)
+    if out is None:
+        out = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    elif out.shape != x.shape or out.dtype != x.dtype or out.device != x.device:
+        raise ValueError("out must be %s %s on %s" % (tuple(x.shape), x.dtype, x.device))
+    o = _matrices("out", out, False)
+    cfg = _cfg(v, steps, coefficients, eps, scale, precision)
+    here, stream = on_device(x)
+    with here:
+        ws = _workspace(cfg, x.device)
+        check(lib().dsvc_orthogonalize(ctypes.byref(cfg), v.data_ptr(), v.stride(1), v.stride(0), o.data_ptr(), o.stride(1), o.stride(0), ws.data_ptr(),
+                                       ws.numel(), stream))
+    return out
+
+
+@torch.no_grad()
+def muon_step_(param, grad, momentum_buffer, lr, momentum=0.95, nesterov=True, weight_decay=0.0, scale=1.0, steps=5, coefficients=COEFFICIENTS, eps=1e-7,
+               precision=None, grad_scale=None):
+    """One step of every matrix of param [..., rows, cols], in place:
+
+      g = grad * grad_scale;  m <- momentum m + (1 - momentum) g;  u = nesterov ? momentum m + (1 - momentum) g : m
+      param <- (1 - lr weight_decay) param - lr * scale * orthogonalize(u)
+
+    momentum_buffer is float32; grad has param's type.  grad_scale: a number or a one-element float32 device tensor (a clip coefficient)."""
+    _check("param", param)
+    if grad.shape != param.shape or grad.dtype != param.dtype or grad.device != param.device:
+        raise ValueError("grad must be %s %s on %s" % (tuple(param.shape), param.dtype, param.device))
+    if momentum_buffer.shape != param.shape or momentum_buffer.dtype != torch.float32 or momentum_buffer.device != param.device:
+        raise ValueError("momentum_buffer must be %s float32 on %s" % (tuple(param.shape), param.device))
+    dev_scale, num_scale = None, 1.0
+    if torch.is_tensor(grad_scale):
+        if grad_scale.dtype != torch.float32 or grad_scale.numel() != 1 or grad_scale.device != param.device:
+            raise ValueError("grad_scale must be a number or one float32 on %s" % param.device)
+        dev_scale = grad_scale.data_ptr()
+    elif grad_scale is not None:
+        num_scale = float(grad_scale)
+    p, g, m = _matrices("param", param, False), _matrices("grad", grad, True), _matrices("momentum_buffer", momentum_buffer, False)
+    cfg = _cfg(p, steps, coefficients, eps, scale, precision)
+    here, stream = on_device(param)
+    with here:
+        ws = _workspace(cfg, param.device)
+        check(lib().dsvc_muon_step(ctypes.byref(cfg), p.data_ptr(), p.stride(1), p.stride(0), g.data_ptr(), g.stride(1), g.stride(0), m.data_ptr(), m.stride(1),
+                                   m.stride(0), lr, momentum, nesterov, weight_decay, dev_scale, num_scale, ws.data_ptr(), ws.numel(), stream))
+    return param

@@ -1,0 +1,157 @@
+"""Token embedding on the HIP kernels: lookup with scaling and its gradient by sorted tokens (csrc/embed.hip) -- what the reference's embedding
+tables do through ``nn.Embedding`` and its autograd (modules/fastspeech/fs2.py:73,81-82,240-247).
+
+  * ``embed_tokens(tokens, weight, scale, padding_idx)``   y[i] = scale * weight[tokens[i]], differentiable in ``weight``
+  * ``embed_tokens_grad(tokens, dy, vocab, ...)``          dW[v] (+)= scale * sum of dy over the places of token v
+  * ``TokenEmbeddingHip``                                  the module: an ``nn.Embedding`` (same parameters, same state dict)
+
+Tables and gradients are float32, float16 or bfloat16; tokens int32 or int64 of any shape.  Sums run in float32 in a fixed order: the gradient is
+bit-identical from call to call.  A token outside [0, vocab) gives a zero row and no gradient; a sticky device flag records it
+(``TokenEmbeddingHip.check()`` raises the IndexError that ``nn.Embedding`` would have raised)."""
+import ctypes
+
+import torch
+from torch import nn
+
+from . import _lib
+from ._lib import check, lib
+
+DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def on_device(t):
+    """(context that makes t's device the current one, the raw handle of that device's current stream)."""
+    i = t.device.index
+    return torch.cuda.device(i) if i != torch.cuda.current_device() else _here, torch._C._cuda_getCurrentRawStream(i)
+
+
+class _Here:
+    def __enter__(self):
+        pass
+
+    def __exit__(self, *exc):
+        return False
+
+
+_here = _Here()
+
+
+def rows_of(t):
+    """t with unit stride along its rows and rows that do not overlap (a copy where they do), for a 2-d tensor."""
+    return t if (t.shape[1] <= 1 or t.stride(1) == 1) and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1]) else t.contiguous()
+
+
+def _check_tokens(tokens, other):
+    if tokens.dtype not in (torch.int64, torch.int32):
+        raise TypeError("diffsvc_amd: tokens must be int32 or int64, got %s" % tokens.dtype)
+    if not other.is_cuda or tokens.device != other.device:
+        raise RuntimeError("diffsvc_amd: tokens (%s) and tensors (%s) must live on one HIP device; there is no CPU path" % (tokens.device, other.device))
+
+
+def _padding(padding_idx, vocab):
+    if padding_idx is None:
+        return -1
+    if not -vocab <= padding_idx < vocab:
+        raise ValueError("padding_idx %d outside a table of %d rows" % (padding_idx, vocab))
+    return padding_idx % vocab
+
+
+def _lookup(tokens, weight, scale, flag):
+    if weight.dim() != 2 or not weight.shape[0] or not weight.shape[1]:
+        raise ValueError("the table must be [rows, columns], got %s" % (tuple(weight.shape),))
+    if weight.dtype not in DTYPES:
+        raise TypeError("diffsvc_amd: tables are float32, float16 or bfloat16, got %s" % weight.dtype)
+    _check_tokens(tokens, weight)
+    V, H = weight.shape
+    w, t = rows_of(weight), tokens if tokens.is_contiguous() else tokens.contiguous()
+    out = torch.empty(tokens.shape + (H,), device=w.device, dtype=w.dtype)
+    here, stream = on_device(w)
+    with here:
+        check(lib().dsvc_embed_tokens(t.data_ptr(), t.dtype == torch.int64, t.numel(), w.data_ptr(), w.stride(0), V, H, DTYPES[w.dtype], scale,
+                                      out.data_ptr(), H, None if flag is None else flag.data_ptr(), stream))
+    return out
+
+
+def embed_tokens_grad(tokens, dy, vocab, scale=1.0, padding_idx=None, out=None, accumulate=False):
+    """Gradient of ``embed_tokens`` in its table, [vocab, H]: dy is [..., H] over tokens of shape [...].  ``out`` (dy's type or float32) is
+    written whole, zeros where a token does not occur; with ``accumulate`` the sums are added to what it holds instead."""
+    if dy.dtype not in DTYPES:
+        raise TypeError("diffsvc_amd: gradients are float32, float16 or bfloat16, got %s" % dy.dtype)
+    if dy.dim() < 1 or tuple(dy.shape[:-1]) != tuple(tokens.shape) or not dy.shape[-1]:
+        raise ValueError("shape mismatch: tokens %s, gradient %s" % (tuple(tokens.shape), tuple(dy.shape)))
+    if vocab < 1:
+        raise ValueError("a table of %d rows" % vocab)
+    _check_tokens(tokens, dy)
+    H, n = dy.shape[-1], tokens.numel()
+    pad = _padding(padding_idx, vocab)
+    d = dy if dy.dim() == 2 else dy.reshape(n, H)
+    d, t = rows_of(d), tokens if tokens.is_contiguous() else tokens.contiguous()
+    if out is None:
+        if accumulate:
+            raise ValueError("accumulate needs the tensor to add to (out)")
+        out = torch.empty(vocab, H, device=d.device, dtype=d.dtype)
+    elif tuple(out.shape) != (vocab, H) or out.device != d.device or out.dtype not in (d.dtype, torch.float32):
+        raise ValueError("out must be [%d, %d] of %s or float32 on %s" % (vocab, H, d.dtype, d.device))
+    elif (H > 1 and out.stride(1) != 1) or (vocab > 1 and out.stride(0) < H):
+        raise ValueError("out needs rows of unit stride that do not overlap, got strides %s" % (out.stride(),))
+    here, stream = on_device(d)
+    with here:
+        need = ctypes.c_int64(0)
+        check(lib().dsvc_embed_tokens_grad_workspace(n, vocab, H, ctypes.byref(need)))
+        ws = torch.empty(need.value, device=d.device, dtype=torch.uint8)
+        check(lib().dsvc_embed_tokens_grad(t.data_ptr(), t.dtype == torch.int64, n, d.data_ptr(), d.stride(0), DTYPES[d.dtype], vocab, H, scale, pad,
+                                           out.data_ptr(), out.stride(0), DTYPES[out.dtype], accumulate, ws.data_ptr(), need.value, stream))
+    return out
+
+
+class _EmbedTokens(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, tokens, weight, scale, padding_idx, flag):
+        ctx.save_for_backward(tokens)
+        ctx.args = weight.shape[0], scale, padding_idx
+        return _lookup(tokens, weight, scale, flag)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        vocab, scale, padding_idx = ctx.args
+        return None, embed_tokens_grad(ctx.saved_tensors[0], dy, vocab, scale, padding_idx), None, None, None
+
+
+def embed_tokens(tokens, weight, scale=1.0, padding_idx=None, flag=None):
+    """scale * weight[tokens], [..., H] for tokens [...]; differentiable in ``weight``, whose row ``padding_idx`` gets no gradient.  flag: an int32
+    device tensor that is set to 1 where a token lies outside the table (its row is zero)."""
+    scale = float(scale)
+    if padding_idx is not None:
+        padding_idx = _padding(padding_idx, weight.shape[0])
+    if flag is not None and (flag.dtype != torch.int32 or flag.device != weight.device or flag.numel() < 1):
+        raise ValueError("flag must be an int32 tensor on %s" % weight.device)
+    if weight.requires_grad and torch.is_grad_enabled():
+        return _EmbedTokens.apply(tokens, weight, scale, padding_idx, flag)
+    return _lookup(tokens, weight, scale, flag)
+
+
+class TokenEmbeddingHip(nn.Embedding):
+    """``nn.Embedding`` whose device path runs on the HIP kernels, with an output scale.  Host tensors take ``nn.Embedding``'s own path."""
+
+    def __init__(self, num_embeddings, embedding_dim, padding_idx=None, scale=1.0, **kw):
+        for k in ("max_norm", "scale_grad_by_freq", "sparse"):
+            if kw.get(k):
+                raise NotImplementedError("TokenEmbeddingHip: %s" % k)
+        super().__init__(num_embeddings, embedding_dim, padding_idx, **kw)
+        self.scale = float(scale)
+        self._flag = None              # sticky device flag: a token outside the table (check)
+
+    def forward(self, tokens):
+        if not self.weight.is_cuda:
+            y = super().forward(tokens)
+            return y * self.scale if self.scale != 1.0 else y
+        if self._flag is None or self._flag.device != self.weight.device:
+            self._flag = torch.zeros(1, device=self.weight.device, dtype=torch.int32)
+        return embed_tokens(tokens, self.weight, self.scale, self.padding_idx, self._flag)
+
+    def check(self):
+        """Raise IndexError if a lookup on the device since the last check was given a token outside the table.  Synchronises."""
+        if self._flag is not None and int(self._flag.item()):
+            self._flag.zero_()
+            raise IndexError("diffsvc_amd: a token lies outside [0, %d); its row was zero" % self.num_embeddings)

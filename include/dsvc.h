@@ -372,6 +372,50 @@ DSVC_API int dsvc_adamw_step(float* params, const float* grads, float* exp_avg, 
 /* clip_grad_norm_: *sqnorm_dev <- ||g||^2, *coef_dev <- min(1, max_norm / (||g|| + 1e-6)) */
 DSVC_API int dsvc_grad_clip_coef(const float* grads, int64_t n, float max_norm, float* sqnorm_dev, float* coef_dev, void* stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * Token embedding (torch.nn.Embedding of modules/fastspeech/fs2.py:73,81-82,240-247 and its autograd) and the orthogonalised update of
+ * matrix parameters.  Tensors of these entry points are fp32, fp16 or bf16 (DSVC_DTYPE_*), rows of stride-1 elements with a row stride `ld` and,
+ * for batches, a matrix stride `bs`, in elements.  Scratch memory is the caller's: the workspace is written and read by the call's own kernels
+ * only, needs no initialisation, starts on 256 bytes, and must stay untouched until the work on `stream` is done; calls that run at the same
+ * time need one each.  Nothing is retained: any of these calls may be captured into a HIP graph.
+ * ---------------------------------------------------------------------------------------------- */
+enum { DSVC_DTYPE_F32 = 0, DSVC_DTYPE_F16 = 1, DSVC_DTYPE_BF16 = 2 };
+
+/* out[i][0..H) = scale * table[tokens[i]][0..H), the product in fp32, rounded once.  tokens: int64 (tokens_i64 != 0) or int32, device.  A token
+ * outside [0, vocab) gives a zero row and sets *out_of_range (device int32, may be NULL) to 1; it is never cleared here. */
+DSVC_API int dsvc_embed_tokens(const void* tokens, int32_t tokens_i64, int64_t n, const void* table, int64_t table_ld, int64_t vocab, int32_t H, int32_t dtype,
+                               float scale, void* out, int64_t out_ld, int32_t* out_of_range, void* stream);
+/* dw[v] (+)= scale * sum of dy[i] over the places i with tokens[i] == v, in fp32 in a fixed order (bit-identical from call to call), rounded once;
+ * accumulate == 0 overwrites all vocab rows (zeros where a token does not occur), else adds to the rows that occur.  padding_idx (a negative
+ * value: none) and tokens outside [0, vocab) contribute nothing.  dw has dy's type or fp32. */
+DSVC_API int dsvc_embed_tokens_grad_workspace(int64_t n, int64_t vocab, int32_t H, int64_t* bytes);
+DSVC_API int dsvc_embed_tokens_grad(const void* tokens, int32_t tokens_i64, int64_t n, const void* dy, int64_t dy_ld, int32_t dy_dtype, int64_t vocab, int32_t H,
+                                    float scale, int64_t padding_idx, void* dw, int64_t dw_ld, int32_t dw_dtype, int32_t accumulate, void* workspace,
+                                    int64_t workspace_bytes, void* stream);
+
+typedef struct {
+    int32_t dtype;            /* DSVC_DTYPE_* of the tensor(s) */
+    int32_t planes;           /* fp16 planes per operand of the products: 1, 2 (fp32-class) or 0 = 1 for bf16, else 2 */
+    int32_t batch, rows, cols;
+    int32_t steps;            /* 1 ... 64 */
+    float coef[3];            /* a, b, c: one step takes a singular value s to s (a + b s^2 + c s^4) */
+    float eps;                /* X = G / (||G||_F + eps) */
+    float scale;              /* of the result */
+} dsvc_ortho_cfg;
+
+/* out = scale * (Newton-Schulz iteration of in / (||in||_F + eps)), each matrix of the batch on its own; out may be in.  Coefficients whose
+ * iterates leave fp16's range from singular values in [0, 1] are refused. */
+DSVC_API int dsvc_ortho_workspace(const dsvc_ortho_cfg* cfg, int64_t* bytes);
+DSVC_API int dsvc_orthogonalize(const dsvc_ortho_cfg* cfg, const void* in, int64_t in_ld, int64_t in_bs, void* out, int64_t out_ld, int64_t out_bs,
+                                void* workspace, int64_t workspace_bytes, void* stream);
+/* One optimisation step of a batch of equally shaped matrices, all in place:
+ *   g = grad * (*grad_scale_dev, or grad_scale where that is NULL);  m <- mu m + (1 - mu) g;  u = nesterov ? mu m + (1 - mu) g : m
+ *   param <- (1 - lr weight_decay) param - lr * cfg->scale * orthogonalised u
+ * param and grad have cfg->dtype, momentum is fp32.  Workspace as dsvc_orthogonalize. */
+DSVC_API int dsvc_muon_step(const dsvc_ortho_cfg* cfg, void* param, int64_t param_ld, int64_t param_bs, const void* grad, int64_t grad_ld, int64_t grad_bs,
+                            float* momentum, int64_t momentum_ld, int64_t momentum_bs, float lr, float mu, int32_t nesterov, float weight_decay,
+                            const float* grad_scale_dev, float grad_scale, void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
