@@ -58,6 +58,7 @@ __device__ __forceinline__ void pack_w_body(const PackDesc& d, long long first, 
         float w = 0.f;
         if (col >= 0 && col < d.cout && ci < d.cin)
             w = d.src[(long long)col * d.s_col + (long long)ci * d.s_ci + (long long)(d.flip ? d.taps - 1 - tap : tap) * d.s_tap] * d.scale;
+        w = one_value(w);
         const _Float16 hi = (_Float16)w;
         _Float16* f = d.dst + ((((size_t)ct * d.taps + tap) * nk16 + k) * 2) * 512 + l * 8 + e;
         f[0] = hi;

@@ -72,6 +72,14 @@ __device__ inline void philox_normal4(uint32_t c0, uint32_t c1, uint32_t c2, uin
     out[2] = rb * c; out[3] = rb * s;
 }
 
+// v as the fp32 number it is.  An fp16 split hi = fp16(v), lo = fp16(v - hi) needs ONE v: left alone, hipcc may fold the multiplication that made v
+// into one of the conversions (v_fma_mixlo_f16: rounded once, from the exact product) and not into the other (v_mul_f32, then v_cvt: twice).
+// On a tie the stored hi and the one that lo is taken from then differ by an fp16 step, which is 2^-11 of v lost.  Costs no instruction.
+__device__ __forceinline__ float one_value(float v) {
+    asm("" : "+v"(v));
+    return v;
+}
+
 inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
 inline int round_up(int a, int b) { return ceil_div(a, b) * b; }
 

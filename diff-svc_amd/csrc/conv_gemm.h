@@ -212,7 +212,7 @@ conv_gemm_kernel(const ConvGemmArgs a, const typename Epi::Args ea) {
                 }
                 half8 hi;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) hi[j] = (_Float16)v[j];
+                for (int j = 0; j < 8; ++j) { v[j] = one_value(v[j]); hi[j] = (_Float16)v[j]; }
                 *reinterpret_cast<half8*>(xs + rr * XS + c8) = hi;
                 if constexpr (NA == 2) {
                     half8 lo;

@@ -324,6 +324,7 @@ __global__ void k_plms(const PlmsArgs a) {
             const size_t row = i / (size_t)a.M;
             if (a.rowclip[row] >= 0) {
                 const int c = (int)(i - row * (size_t)a.M);
+                xn = one_value(xn);
                 const _Float16 h = (_Float16)xn;
                 _Float16* q = a.xsh + row * (size_t)(2 * a.ldh) + c;
                 q[0] = h;

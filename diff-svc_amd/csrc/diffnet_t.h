@@ -74,7 +74,7 @@ struct TEpiGate {
             half8 o, ol;
 #pragma unroll
             for (int r = 0; r < 8; ++r) {
-                const float v = gate_act_scaled(acc[nt][r], acc[nt][8 + r]);
+                const float v = one_value(gate_act_scaled(acc[nt][r], acc[nt][8 + r]));
                 o[r] = (_Float16)v;
                 ol[r] = (_Float16)(v - (float)o[r]);
             }

@@ -140,7 +140,7 @@ __global__ __launch_bounds__(256) void k_ns_prep(const void* __restrict__ in, Vi
         half8 hi, lo;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const float v = q < 8 ? tile[row][k + e] : tile[k + e][row];
+            const float v = one_value(q < 8 ? tile[row][k + e] : tile[k + e][row]);
             hi[e] = (_Float16)v;
             lo[e] = (_Float16)(v - (float)hi[e]);
         }
@@ -375,6 +375,7 @@ __global__ __launch_bounds__(WR * WC * 64) void k_ns_gemm(const NsGemm g) {
                         v = fmaf(g.c1, am, v);
                         if (bi == bj && 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3) == (lane & 31)) v += g.c0;
                     }
+                    v = one_value(v);
                     hi[r >> 2][r & 3] = (_Float16)v;
                     if (P == 2) lo[r >> 2][r & 3] = (_Float16)(v - (float)hi[r >> 2][r & 3]);
                 }

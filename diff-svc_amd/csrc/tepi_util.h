@@ -29,8 +29,9 @@ __device__ __forceinline__ void store_hi_lo16(_Float16* dst, int lo_off, const f
     half8 h0, h1, l0, l1;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        h0[i] = (_Float16)v[i]; h1[i] = (_Float16)v[8 + i];
-        l0[i] = (_Float16)(v[i] - (float)h0[i]); l1[i] = (_Float16)(v[8 + i] - (float)h1[i]);
+        const float a = one_value(v[i]), b = one_value(v[8 + i]);
+        h0[i] = (_Float16)a; h1[i] = (_Float16)b;
+        l0[i] = (_Float16)(a - (float)h0[i]); l1[i] = (_Float16)(b - (float)h1[i]);
     }
     *reinterpret_cast<half8*>(dst) = h0;
     *reinterpret_cast<half8*>(dst + 8) = h1;

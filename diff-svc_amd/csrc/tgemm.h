@@ -757,7 +757,7 @@ static __global__ void k_tpack(const float* __restrict__ src, const int* __restr
         const int row = mt * 32 + (l & 31), ci = k * 16 + 8 * (l >> 5) + e;
         const int o = rowmap[row];
         const int cs = fold > 0 ? ci % fold : ci;          // fold: input channels [fold, 2*fold) repeat [0, fold) -- the lo plane of a
-        const float w = (o >= 0 && cs < I) ? src[((size_t)o * I + cs) * taps + tap] * scale * (rowscale ? rowscale[row] : 1.0f) : 0.f;   // split activation sees the same weights
+        const float w = one_value((o >= 0 && cs < I) ? src[((size_t)o * I + cs) * taps + tap] * scale * (rowscale ? rowscale[row] : 1.0f) : 0.f);   // split activation sees the same weights
         _Float16 hi;
         if (n_variants > 1) {
             int vr = 0;
@@ -832,7 +832,7 @@ static __global__ void k_tpack6(const float* __restrict__ src, const int* __rest
         unsigned out[6];
         for (int m = 0; m < 32; ++m) {
             const int ci = 64 * q + 16 * (m >> 3) + 8 * h + (m & 7);
-            const float w = (o >= 0 && ci < I) ? src[((size_t)o * I + ci) * taps + tap] * scale * (rowscale ? rowscale[row] : 1.0f) : 0.f;
+            const float w = one_value((o >= 0 && ci < I) ? src[((size_t)o * I + ci) * taps + tap] * scale * (rowscale ? rowscale[row] : 1.0f) : 0.f);
             const float wl = whole ? w : w - (float)(_Float16)w;
             const float u = wl * inv6, a = fabsf(u);
             int i0 = tg_e2m3_floor(a);

@@ -142,7 +142,7 @@ struct TEpiGateT {
                 const float e1 = __builtin_amdgcn_exp2f(acc[nt][r]), e2 = __builtin_amdgcn_exp2f(bf);
                 s[r] = __builtin_amdgcn_rcpf(1.0f + e1);
                 t[r] = (1.0f - e2) * __builtin_amdgcn_rcpf(1.0f + e2);
-                gv[r] = ok ? s[r] * t[r] : 0.f;
+                gv[r] = one_value(ok ? s[r] * t[r] : 0.f);
             }
             const size_t o = (size_t)frame * e.C + cg;
             st4(e.sig + o, f32x4{s[0], s[1], s[2], s[3]}); st4(e.sig + o + 4, f32x4{s[4], s[5], s[6], s[7]});
@@ -351,7 +351,8 @@ __global__ void k_tpack_batch(const TPackDesc* __restrict__ descs) {
         const int mt = (int)(r / d.taps);
         const int row = mt * 32 + (l & 31), ci = k * 16 + 8 * (l >> 5) + e;
         const int o = d.rowmap[row];
-        const float w = (o >= 0 && ci < d.I) ? d.src[o * d.s_o + ci * d.s_i + (d.flip ? d.taps - 1 - tap : tap) * d.s_tap] * (d.rowscale ? d.rowscale[row] : 1.0f) : 0.f;
+        float w = (o >= 0 && ci < d.I) ? d.src[o * d.s_o + ci * d.s_i + (d.flip ? d.taps - 1 - tap : tap) * d.s_tap] * (d.rowscale ? d.rowscale[row] : 1.0f) : 0.f;
+        w = one_value(w);
         const _Float16 hi = (_Float16)w;
         _Float16* f = d.dst + ((((size_t)mt * d.taps + tap) * nk16 + k) * 2) * 512 + l * 8 + e;
         f[0] = hi;

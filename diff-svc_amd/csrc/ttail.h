@@ -139,8 +139,9 @@ ttail_kernel(const TTailArgs a) {
         half8 h0, h1, l0, l1;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            h0[i] = (_Float16)v[i]; h1[i] = (_Float16)v[8 + i];
-            l0[i] = (_Float16)(v[i] - (float)h0[i]); l1[i] = (_Float16)(v[8 + i] - (float)h1[i]);
+            const float a = one_value(v[i]), b = one_value(v[8 + i]);
+            h0[i] = (_Float16)a; h1[i] = (_Float16)b;
+            l0[i] = (_Float16)(a - (float)h0[i]); l1[i] = (_Float16)(b - (float)h1[i]);
         }
         const unsigned rowb = tile0 + (unsigned)f * rb, sw = (unsigned)(f & 15);
         const unsigned c0 = (unsigned)(cb >> 3);

@@ -322,7 +322,7 @@ k_pair_mfma(const float* __restrict__ x, float* __restrict__ out, const _Float16
             }
             half8 hi, lo;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) { hi[e] = (_Float16)v[e]; lo[e] = (_Float16)(v[e] - (float)hi[e]); }
+            for (int e = 0; e < 8; ++e) { v[e] = one_value(v[e]); hi[e] = (_Float16)v[e]; lo[e] = (_Float16)(v[e] - (float)hi[e]); }
             *reinterpret_cast<half8*>(lds + r * XS + c8) = hi;
             *reinterpret_cast<half8*>(lds + xplane + r * XS + c8) = lo;
         }
@@ -385,6 +385,7 @@ k_pair_mfma(const float* __restrict__ x, float* __restrict__ out, const _Float16
                         float v = acc[m][n][4 * q + e] + bb[e];
                         v = v > 0.f ? v : 0.1f * v;
                         if (!ok) v = 0.f;
+                        v = one_value(v);
                         hi[e] = (_Float16)v;
                         lo[e] = (_Float16)(v - (float)hi[e]);
                     }
@@ -799,6 +800,7 @@ __global__ void k_lrelu_planes(const float* __restrict__ x, _Float16* __restrict
         _Float16* q = ph + (size_t)row * (2 * C) + c4;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
+            v[j] = one_value(v[j]);
             const _Float16 h = (_Float16)v[j];
             q[j] = h;
             q[C + j] = (_Float16)(v[j] - (float)h);
