@@ -36,7 +36,7 @@ typedef const half8 __attribute__((address_space(3))) * lds_half8;
 
 constexpr float X_SCALE = 4096.f, A_SCALE = 1024.f;
 constexpr int PAD = 128;                     // rows and columns of every intermediate are padded to this
-constexpr int SUM_BLOCKS = 128;              // partial sums of squares per matrix
+constexpr int SUM_BLOCKS = 256;              // partial sums of squares per matrix
 
 enum { F32 = DSVC_DTYPE_F32, F16 = DSVC_DTYPE_F16, BF16 = DSVC_DTYPE_BF16 };
 
@@ -63,28 +63,52 @@ __device__ __forceinline__ float muon_mom(const MuonArgs& u, float g, float m) {
 __device__ __forceinline__ float muon_u(const MuonArgs& u, float g, float m) { return u.nesterov ? fmaf(u.mu, m, (1.f - u.mu) * g) : m; }
 
 // ---- sums of squares (fp64), and the momentum update on the way: grid (blocks, matrices).  Partials are combined in a fixed order. ----
-template <int T, bool MUON>
-__global__ __launch_bounds__(256) void k_ns_sums(const void* __restrict__ in, View iv, int rows, int cols, MuonArgs mu, double* __restrict__ part,
+// flat: rows follow one another without gaps in every tensor (one row of rows * cols elements); vec: every row start and the row length allow
+// 16-byte accesses of VEC elements
+template <int T, bool MUON, int VEC>
+__global__ __launch_bounds__(256) void k_ns_sums(const void* __restrict__ in, View iv, int rows, long long cols, MuonArgs mu, double* __restrict__ part,
                                                  int* __restrict__ count, int n_count) {
     typedef typename Elem<T>::type E;
+    typedef E EV __attribute__((ext_vector_type(VEC)));
+    typedef float FV __attribute__((ext_vector_type(VEC)));
     const int b = blockIdx.y;
     const E* src = (const E*)in + b * iv.bs;
     float* mom = MUON ? mu.mom + b * mu.mv.bs : nullptr;
     const float gs = MUON ? (mu.gscale_dev ? *mu.gscale_dev : mu.gscale) : 1.f;
     for (int i = (blockIdx.y * gridDim.x + blockIdx.x) * 256 + threadIdx.x; i < n_count; i += gridDim.x * gridDim.y * 256) count[i] = 0;
-    const long long n = (long long)rows * cols;
+    const long long per_row = cols / VEC, n = rows * per_row, step = (long long)gridDim.x * 256;
     double s = 0.0;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
-        const int r = (int)(i / cols), c = (int)(i - (long long)r * cols);
-        float v = (float)src[r * iv.ld + c];
-        if (MUON) {
-            const float g = v * gs;
-            float* p = mom + r * mu.mv.ld + c;
-            const float m = muon_mom(mu, g, *p);
-            *p = m;
-            v = muon_u(mu, g, m);
+    for (long long i0 = (long long)blockIdx.x * 256 + threadIdx.x; i0 < n; i0 += 4 * step) {
+        EV v[4];
+        FV m[4];
+        long long at[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const long long i = i0 + k * step;
+            if (i >= n) continue;
+            const long long r = rows == 1 ? 0 : (unsigned long long)i < (1ull << 32) && per_row < (1ll << 32) ? (unsigned)i / (unsigned)per_row : i / per_row;
+            const long long c = (i - r * per_row) * VEC;
+            v[k] = *(const EV*)(src + r * iv.ld + c);
+            if (MUON) {
+                at[k] = r * mu.mv.ld + c;
+                m[k] = *(const FV*)(mom + at[k]);
+            }
         }
-        s += (double)v * (double)v;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (i0 + k * step >= n) continue;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                float x = (float)v[k][e];
+                if (MUON) {
+                    x *= gs;
+                    m[k][e] = muon_mom(mu, x, m[k][e]);
+                    x = muon_u(mu, x, m[k][e]);
+                }
+                s = fma((double)x, (double)x, s);
+            }
+            if (MUON) *(FV*)(mom + at[k]) = m[k];
+        }
     }
     __shared__ double red[256];
     red[threadIdx.x] = s;
@@ -102,11 +126,11 @@ __global__ __launch_bounds__(256) void k_ns_prep(const void* __restrict__ in, Vi
                                                  int n_part, double eps, _Float16* __restrict__ x, _Float16* __restrict__ xt, int mp, int np, Scalars* __restrict__ sc) {
     typedef typename Elem<T>::type E;
     const int b = blockIdx.z, i0 = blockIdx.y * 64, j0 = blockIdx.x * 64, tid = threadIdx.x;
-    __shared__ double red[128];
+    __shared__ double red[SUM_BLOCKS];
     __shared__ float tile[64][65];
-    if (tid < 128) red[tid] = tid < n_part ? part[(long long)b * n_part + tid] : 0.0;
+    red[tid] = tid < n_part ? part[(long long)b * n_part + tid] : 0.0;
     __syncthreads();
-    for (int k = 64; k > 0; k >>= 1) {
+    for (int k = SUM_BLOCKS / 2; k > 0; k >>= 1) {
         if (tid < k) red[tid] += red[tid + k];
         __syncthreads();
     }
@@ -158,7 +182,8 @@ struct NsGemm {
     const _Float16 *a, *b;                   // fragment-order operands, rows x K each: result[i][j] = sum_k a[i][k] b[j][k]
     long long a_bs, b_bs;                    // halfs per matrix
     int nk16;                                // K / 16
-    int tiles_i, tiles_j, n_tiles, batch, slices;
+    int tiles_i, n_tiles;                    // tiles along i, tiles of a matrix
+    int full, rest, slices;                  // of all matrices' tiles: the first `full` in one piece, the `rest` in `slices` pieces of K each
     float* part; int* count;                 // split K: partial tiles and arrival counters
     _Float16 *o, *ot;                        // FULL: result (k = j), transposed result (k = i); GRAM / POLY: ot only (symmetric)
     long long o_bs, ot_bs;
@@ -200,19 +225,41 @@ __device__ __forceinline__ void transpose_tile(const half4 (&v)[4], const half8 
     for (int r = 0; r < 16; ++r) t[r >> 2][r & 3] = (_Float16)acc[r];
 }
 
-// One workgroup = a tile of (32 TM WR) x (32 TN WC) of one matrix (or one K slice of it); WR x WC waves of TM x TN accumulator tiles; NST stages of
-// KS k steps in LDS.
-template <int P, int TM, int TN, int WR, int WC, int KS, int NST, int MODE>
-__global__ __launch_bounds__(WR * WC * 64) void k_ns_gemm(const NsGemm g) {
-    constexpr int NW = WR * WC, RA = TM * WR, RB = TN * WC, U = KS * P, PIECES = (RA + RB) * U, PER = PIECES / NW;
+// One workgroup = a tile of (32 TM WR) x (32 TN WC) of one matrix (or one K slice of it): G groups of WR x WC waves, a wave = TM x TN accumulator
+// tiles; NST stages of KS k steps in LDS, the groups take every G-th k step of a stage and are added up at the end.
+template <int P_, int TM_, int TN_, int WR_, int WC_, int G_, int KS_, int NST_, int PER_CU_>
+struct Tile {
+    static constexpr int P = P_, TM = TM_, TN = TN_, WR = WR_, WC = WC_, G = G_, KS = KS_, NST = NST_, PER_CU = PER_CU_;
+    static constexpr int NW = WR * WC * G, RA = TM * WR, RB = TN * WC, U = KS * P, PIECES = (RA + RB) * U, PER = PIECES / NW;
+    static constexpr int LDS_STAGES = PIECES * NST * 1024, LDS_JOIN = (G - 1) * WR * WC * TM * TN * 4096;
+    static constexpr int LDS = LDS_STAGES > LDS_JOIN ? LDS_STAGES : LDS_JOIN;
+    static_assert(PIECES % NW == 0 && KS % G == 0 && PER * (NST - 2) < 64 && LDS * PER_CU <= 160 * 1024, "");
+};
+
+template <class C, int MODE>
+__global__ __launch_bounds__(C::NW * 64) void k_ns_gemm(const NsGemm g) {
+    constexpr int P = C::P, TM = C::TM, TN = C::TN, WC = C::WC, KS = C::KS, NST = C::NST, NW = C::NW, RA = C::RA, RB = C::RB, U = C::U, PIECES = C::PIECES, PER = C::PER;
+    constexpr int WAVES = C::WR * C::WC, TILE4 = TM * TN * 4 * WAVES * 64;         // waves of a group; f32x4 of a tile
     constexpr bool SYM = MODE == GRAM || MODE == POLY;
-    static_assert(PIECES % NW == 0 && PER * (NST - 2) < 64, "");
+    constexpr int CHAINS = TM * TN == 1 && P == 2 ? 3 : 1;                         // one accumulator tile: the three products run as chains of their own
     extern __shared__ __attribute__((aligned(1024))) char smem[];
-    // workgroups of one XCD (id % 8) take neighbouring tiles: they share operand rows in its L2
-    const int total = g.batch * g.n_tiles * g.slices, per = (total + 7) / 8;
-    const int lin = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-    if ((int)(blockIdx.x >> 3) >= per || lin >= total) return;
-    const int tile = lin % g.n_tiles, bs = lin / g.n_tiles, slice = bs % g.slices, b = bs / g.slices;
+    // workgroups of one XCD (id % 8) take neighbouring tiles: they share operand rows in its L2, and the slices of a tile meet there
+    int at, slice = 0, slices = 1;
+    {
+        const int first = (g.full + 7) & ~7, id = blockIdx.x;
+        if (id < first) {
+            at = (id & 7) * (first >> 3) + (id >> 3);
+            if (at >= g.full) return;
+        } else {
+            const int units = g.rest * g.slices, per = (units + 7) >> 3, u = ((id - first) & 7) * per + ((id - first) >> 3);
+            if (u >= units) return;
+            slices = g.slices;
+            at = u / slices;
+            slice = u - at * slices;
+            at += g.full;
+        }
+    }
+    const int b = at / g.n_tiles, tile = at - b * g.n_tiles;
     int ti, tj;
     if (SYM) {
         tj = (int)((sqrtf(8.f * tile + 1.f) - 1.f) * 0.5f);
@@ -224,9 +271,8 @@ __global__ __launch_bounds__(WR * WC * 64) void k_ns_gemm(const NsGemm g) {
         ti = tile - tj * g.tiles_i;
     }
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int wr = wave / WC, wc = wave % WC;
-    const int n_stages_all = g.nk16 / KS, ps = (n_stages_all + g.slices - 1) / g.slices;
-    const int s_begin = slice * ps, n_stages = min(n_stages_all - s_begin, ps);     // (<= 0 for a slice behind the end: contributes zeros)
+    const int grp = wave / WAVES, gw = wave % WAVES, wr = gw / WC, wc = gw % WC;
+    const int all = g.nk16 / KS, s_begin = slice * all / slices, n_stages = (slice + 1) * all / slices - s_begin;
     const _Float16* abase = g.a + b * g.a_bs + (long long)ti * RA * g.nk16 * P * 512;
     const _Float16* bbase = g.b + b * g.b_bs + (long long)tj * RB * g.nk16 * P * 512;
     const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) char*)smem;
@@ -242,13 +288,16 @@ __global__ __launch_bounds__(WR * WC * 64) void k_ns_gemm(const NsGemm g) {
         }
     };
 
-    f32x16 acc[TM][TN];
+    f32x16 acc[TM][TN], more[CHAINS];
 #pragma unroll
-    for (int i = 0; i < TM; ++i)
+    for (int r = 0; r < 16; ++r) {
 #pragma unroll
-        for (int j = 0; j < TN; ++j)
+        for (int i = 0; i < TM; ++i)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+            for (int j = 0; j < TN; ++j) acc[i][j][r] = 0.f;
+#pragma unroll
+        for (int c = 0; c < CHAINS; ++c) more[c][r] = 0.f;
+    }
 
 #pragma unroll
     for (int s = 0; s < NST - 1; ++s)
@@ -260,66 +309,123 @@ __global__ __launch_bounds__(WR * WC * 64) void k_ns_gemm(const NsGemm g) {
         else wait_vm_lgkm<0>();
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        if (s + NST - 1 < n_stages) dma(s + NST - 1);
-        const unsigned buf = lds0 + (unsigned)(s % NST) * (PIECES * 1024) + (unsigned)lane * 16u;
-#pragma unroll
-        for (int k = 0; k < KS; ++k) {
-            half8 fa[TM][P], fb[TN][P];
+        const unsigned buf = lds0 + (unsigned)(s % NST) * (PIECES * 1024) + (unsigned)lane * 16u + (unsigned)(grp * P * 1024);
+        half8 fa[2][TM][P], fb[2][TN][P];
+        auto load = [&](int k) {
 #pragma unroll
             for (int p = 0; p < P; ++p) {
 #pragma unroll
-                for (int i = 0; i < TM; ++i) fa[i][p] = *(lds_half8)(size_t)(buf + (unsigned)(((wr * TM + i) * U + k * P + p) * 1024));
+                for (int i = 0; i < TM; ++i) fa[k & 1][i][p] = *(lds_half8)(size_t)(buf + (unsigned)(((wr * TM + i) * U + k * C::G * P + p) * 1024));
 #pragma unroll
-                for (int j = 0; j < TN; ++j) fb[j][p] = *(lds_half8)(size_t)(buf + (unsigned)(((RA + wc * TN + j) * U + k * P + p) * 1024));
+                for (int j = 0; j < TN; ++j) fb[k & 1][j][p] = *(lds_half8)(size_t)(buf + (unsigned)(((RA + wc * TN + j) * U + k * C::G * P + p) * 1024));
             }
+        };
+        load(0);
+        if (s + NST - 1 < n_stages) dma(s + NST - 1);     // (issued under the latency of the first fragments' reads)
+#pragma unroll
+        for (int k = 0; k < KS / C::G; ++k) {
+            if (k + 1 < KS / C::G) load(k + 1);
 #pragma unroll
             for (int i = 0; i < TM; ++i)
 #pragma unroll
                 for (int j = 0; j < TN; ++j) {
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[i][0], fb[j][0], acc[i][j], 0, 0, 0);
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[k & 1][i][0], fb[k & 1][j][0], acc[i][j], 0, 0, 0);
                     if constexpr (P == 2) {
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[i][1], fb[j][0], acc[i][j], 0, 0, 0);
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[i][0], fb[j][1], acc[i][j], 0, 0, 0);
+                        f32x16& x1 = CHAINS > 1 ? more[1 % CHAINS] : acc[i][j];
+                        f32x16& x2 = CHAINS > 1 ? more[2 % CHAINS] : acc[i][j];
+                        x1 = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[k & 1][i][1], fb[k & 1][j][0], x1, 0, 0, 0);
+                        x2 = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[k & 1][i][0], fb[k & 1][j][1], x2, 0, 0, 0);
                     }
                 }
         }
     }
+    if constexpr (CHAINS > 1) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[0][0][r] += more[1 % CHAINS][r] + more[2 % CHAINS][r];
+    }
 
-    if (g.slices > 1) {
-        // every slice leaves its partial tile; the workgroup that arrives last adds them up in slice order (whoever it is: the same sum)
-        const int slot = (b * g.n_tiles + tile);
-        f32x4* mine = (f32x4*)g.part + ((long long)slot * g.slices + slice) * (TM * TN * 4 * NW * 64) + threadIdx.x;
+    if constexpr (C::G > 1) {
+        f32x4* red = (f32x4*)smem + gw * (TM * TN * 4 * 64) + lane;
+        __syncthreads();                     // every wave is done with the stages
+        if (grp > 0) {
 #pragma unroll
-        for (int i = 0; i < TM; ++i)
+            for (int i = 0; i < TM; ++i)
 #pragma unroll
-            for (int j = 0; j < TN; ++j)
+                for (int j = 0; j < TN; ++j)
 #pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    mine[((i * TN + j) * 4 + q) * (NW * 64)] = f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-        __threadfence();
+                    for (int q = 0; q < 4; ++q)
+                        red[(grp - 1) * TILE4 + ((i * TN + j) * 4 + q) * 64] = f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+        }
         __syncthreads();
+        if (grp == 0) {
+#pragma unroll
+            for (int z = 0; z < C::G - 1; ++z)
+#pragma unroll
+                for (int i = 0; i < TM; ++i)
+#pragma unroll
+                    for (int j = 0; j < TN; ++j)
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            const f32x4 v = red[z * TILE4 + ((i * TN + j) * 4 + q) * 64];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) acc[i][j][4 * q + e] += v[e];
+                        }
+        }
+    }
+
+    if (slices > 1) {
+        // every slice leaves its partial tile; the workgroup that arrives last adds them up in slice order (whoever it is: the same sum).  The partials
+        // go through agent-scope accesses, which pass the XCDs' own L2s: a fence would write a whole L2 back (__threadfence() here made a
+        // [2048, 2048] fp32 call 1.40 instead of 0.89 ms)
+        typedef unsigned long long u64;
+        const int slot = at - g.full;
+        auto part = [&](int z, int x) { return (u64*)g.part + (((long long)slot * slices + z) * TILE4 + x * (WAVES * 64) + threadIdx.x) * 2; };
+        if (grp == 0) {
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const float2 v = make_float2(acc[i][j][4 * q + 2 * h], acc[i][j][4 * q + 2 * h + 1]);
+                            __hip_atomic_store(part(slice, (i * TN + j) * 4 + q) + h, __builtin_bit_cast(u64, v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                        }
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");         // this wave's partials are where every XCD sees them ...
+        __syncthreads();                                         // ... and so are the workgroup's
         int* last = (int*)smem;
         if (threadIdx.x == 0) {
-            const int at = atomicAdd(g.count + slot, 1);
-            *last = at == g.slices - 1;
-            if (at == g.slices - 1) g.count[slot] = 0;           // for the next launch
+            const int n = __hip_atomic_fetch_add(g.count + slot, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            *last = n == slices - 1;
+            if (n == slices - 1) __hip_atomic_store(g.count + slot, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);      // for the next launch
         }
         __syncthreads();
         if (!*last) return;
-        __threadfence();
-        const f32x4* all = (const f32x4*)g.part + (long long)slot * g.slices * (TM * TN * 4 * NW * 64) + threadIdx.x;
+        if (grp == 0) {
 #pragma unroll
-        for (int i = 0; i < TM; ++i)
+            for (int i = 0; i < TM; ++i)
 #pragma unroll
-            for (int j = 0; j < TN; ++j)
+                for (int j = 0; j < TN; ++j)
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    f32x4 v = all[((i * TN + j) * 4 + q) * (NW * 64)];
-                    for (int z = 1; z < g.slices; ++z) v += all[(long long)z * (TM * TN * 4 * NW * 64) + ((i * TN + j) * 4 + q) * (NW * 64)];
+                    for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+            for (int z = 0; z < slices; ++z)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[i][j][4 * q + e] = v[e];
-                }
+                for (int i = 0; i < TM; ++i)
+#pragma unroll
+                    for (int j = 0; j < TN; ++j)
+#pragma unroll
+                        for (int q = 0; q < 4; ++q)
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                const float2 v = __builtin_bit_cast(float2, __hip_atomic_load(part(z, (i * TN + j) * 4 + q) + h, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+                                acc[i][j][4 * q + 2 * h] += v.x;
+                                acc[i][j][4 * q + 2 * h + 1] += v.y;
+                            }
+        }
     }
+    if (grp > 0) return;
 
     // ---- epilogue: register r of a lane = row 8 (r >> 2) + 4 (lane >> 5) + (r & 3), column lane & 31 ----
     const int e0 = g.sc[b].e0, ek = max(0, e0 - g.step * g.dec), ek1 = max(0, e0 - (g.step + 1) * g.dec);
@@ -392,24 +498,79 @@ __global__ __launch_bounds__(WR * WC * 64) void k_ns_gemm(const NsGemm g) {
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------------------------
-template <int P, int MODE>
-int gemm(NsGemm& g, int mi, int nj, hipStream_t st) {
-    constexpr int TM = 2, TN = 2, WR = 2, WC = 2, KS = 4 / P, NST = 2;
-    constexpr int LDS = (TM * WR + TN * WC) * KS * P * 1024 * NST;
-    g.tiles_i = mi / (32 * TM * WR);
-    g.tiles_j = nj / (32 * TN * WC);
-    g.n_tiles = MODE == GRAM || MODE == POLY ? g.tiles_i * (g.tiles_i + 1) / 2 : g.tiles_i * g.tiles_j;
-    auto kernel = k_ns_gemm<P, TM, TN, WR, WC, KS, NST, MODE>;
-    const long long total = (long long)g.batch * g.n_tiles * g.slices;
-    if (total >= (1LL << 24)) return fail(DSVC_EINVAL, "orthogonalize: %lld tiles", total);
-    hipLaunchKernelGGL(kernel, dim3((unsigned)((total + 7) / 8 * 8)), dim3(WR * WC * 64), LDS, st, g);
+// Tiles.  128: 64 x 64 per wave (4 or 8 fragment reads feed 4 or 12 MFMAs), two workgroups a CU hide each other's barriers; stages of 64 (one plane) or
+// 32 (two) k.  256: 128 x 64 per wave, fewer LDS reads per MFMA.  64: a wave has one accumulator tile, four stages ahead; for grids that 128 leaves
+// mostly empty.
+template <int P, int SIZE> struct Tiles;
+template <> struct Tiles<1, 64> { typedef Tile<1, 1, 1, 2, 2, 1, 4, 4, 2> type; };
+template <> struct Tiles<2, 64> { typedef Tile<2, 1, 1, 2, 2, 1, 2, 4, 2> type; };
+template <> struct Tiles<1, 128> { typedef Tile<1, 2, 2, 2, 2, 1, 4, 2, 2> type; };
+template <> struct Tiles<2, 128> { typedef Tile<2, 2, 2, 2, 2, 1, 2, 2, 2> type; };
+template <> struct Tiles<1, 256> { typedef Tile<1, 4, 2, 2, 4, 1, 4, 2, 1> type; };
+
+constexpr int CUS = 256;
+
+// How one product is cut: the tile's edge, and which tiles are split along K.
+struct Cut {
+    int size, tiles_i, n_tiles, full, rest, slices;
+    long long part_bytes() const { return slices > 1 ? (long long)rest * slices * size * size * 4 : 0; }
+};
+// A slice keeps at least 16 stages: a partial tile's way through memory costs about as much as 8 ([4, 1024, 1024] bf16: 253 us whole, 344 us in slices of
+// 8 or more; [100, 4000] fp32: 250 us whole, 124 us in slices of 16; the last 16 of [4096, 4096] bf16's 528 tiles: 1783 -> 1638 us).
+constexpr int MIN_STAGES = 16;
+template <class C>
+Cut cut_for(int size, bool sym, int batch, int mi, int nj, int k16) {
+    Cut c{};
+    c.size = size;
+    c.tiles_i = mi / size;
+    c.n_tiles = sym ? c.tiles_i * (c.tiles_i + 1) / 2 : c.tiles_i * (nj / size);
+    const long long total = (long long)batch * c.n_tiles, slots = C::PER_CU * CUS;
+    c.rest = (int)(total % slots);
+    c.full = (int)(total - c.rest);
+    c.slices = 1;
+    if (c.rest) {
+        const long long by_slots = slots / c.rest, by_work = k16 / C::KS / MIN_STAGES;
+        c.slices = (int)(by_slots < by_work ? by_slots : by_work);
+        if (c.slices > 16) c.slices = 16;
+    }
+    if (c.slices <= 1) { c.slices = 1; c.full = (int)total; c.rest = 0; }
+    return c;
+}
+template <int P>
+Cut cut(bool sym, int batch, int mi, int nj, int k16) {
+    // 128 where that gives every CU a tile ([1000, 3000] fp32 on 36 ... 192 tiles of 128: 665 us, on tiles of 64: 376 us; [768, 384] x 20: 346 -> 282 us;
+    // [2048, 2048]'s symmetric products on 136 tiles in K slices: 869 us, on tiles of 64: 781 us).  256 where it still gives one to each and nothing is
+    // padded for it ([4096, 4096] bf16, the full product: 158 -> 140 us)
+    const int t = mi / 128;
+    const long long tiles = (long long)batch * (sym ? t * (t + 1) / 2 : (long long)t * (nj / 128));
+    if (P == 1 && !sym && mi % 256 == 0 && nj % 256 == 0 && tiles >= 4 * CUS) return cut_for<typename Tiles<1, 256>::type>(256, sym, batch, mi, nj, k16);
+    if (tiles >= CUS) return cut_for<typename Tiles<P, 128>::type>(128, sym, batch, mi, nj, k16);
+    return cut_for<typename Tiles<P, 64>::type>(64, sym, batch, mi, nj, k16);
+}
+
+template <class C, int MODE>
+int launch_gemm(const NsGemm& g, hipStream_t st) {
+    auto kernel = k_ns_gemm<C, MODE>;
+    if (C::LDS > 64 * 1024) DSVC_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS));
+    const int grid = (g.full + 7) / 8 * 8 + (g.rest * g.slices + 7) / 8 * 8;
+    hipLaunchKernelGGL(kernel, dim3(grid), dim3(C::NW * 64), C::LDS, st, g);
     DSVC_HIP(hipGetLastError());
     return DSVC_OK;
+}
+template <int P, int MODE>
+int gemm(NsGemm& g, const Cut& c, hipStream_t st) {
+    g.tiles_i = c.tiles_i; g.n_tiles = c.n_tiles; g.full = c.full; g.rest = c.rest; g.slices = c.slices;
+    if constexpr (P == 1 && (MODE == FULL || MODE == FINAL)) {
+        if (c.size == 256) return launch_gemm<typename Tiles<1, 256>::type, MODE>(g, st);
+    }
+    if (c.size == 128) return launch_gemm<typename Tiles<P, 128>::type, MODE>(g, st);
+    return launch_gemm<typename Tiles<P, 64>::type, MODE>(g, st);
 }
 
 struct Plan {
     int P, m, n, mp, np, tall, n_part, dec;
-    long long off_part, off_sc, off_count, n_count, off_x, off_xt[2], off_a, off_m, bytes;
+    Cut gram, poly, full;
+    long long off_part, off_sc, off_count, n_count, off_split, off_x, off_xt[2], off_a, off_m, bytes;
 };
 
 // The largest singular value that the polynomial can reach from [0, 1] and the largest |a + b s^2 + c s^4| on the way: both stay far from where the
@@ -454,15 +615,30 @@ int make_plan(const dsvc_ortho_cfg* c, Plan* p) {
     if (!c->batch || !p->m) return DSVC_OK;
     p->mp = round_up(p->m, PAD);
     p->np = round_up(p->n, PAD);
-    const long long want = ((long long)p->m * p->n + 4095) / 4096;
+    if ((long long)c->batch * (p->mp / 64) * (p->np / 64) >= (1LL << 22)) return fail(DSVC_EINVAL, "orthogonalize: shape [%d, %d, %d] is too large", c->batch, c->rows, c->cols);
+    if (p->P == 1) {
+        p->gram = cut<1>(true, c->batch, p->mp, p->mp, p->np / 16);
+        p->poly = cut<1>(true, c->batch, p->mp, p->mp, p->mp / 16);
+        p->full = cut<1>(false, c->batch, p->mp, p->np, p->mp / 16);
+    } else {
+        p->gram = cut<2>(true, c->batch, p->mp, p->mp, p->np / 16);
+        p->poly = cut<2>(true, c->batch, p->mp, p->mp, p->mp / 16);
+        p->full = cut<2>(false, c->batch, p->mp, p->np, p->mp / 16);
+    }
+    const long long want = ((long long)p->m * p->n + 8191) / 8192;
     p->n_part = (int)(want < SUM_BLOCKS ? want : SUM_BLOCKS);
     long long at = 0;
     auto take = [&](long long bytes) { const long long o = at; at += (bytes + 1023) / 1024 * 1024; return o; };
     const long long B = c->batch, xs = B * p->mp * p->np * p->P * 2, as = B * p->mp * p->mp * p->P * 2;
     p->off_part = take(B * p->n_part * 8);
     p->off_sc = take(B * (long long)sizeof(Scalars));
-    p->n_count = 0;
+    long long split = 0;
+    for (const Cut* k : {&p->gram, &p->poly, &p->full}) {
+        if (k->rest > p->n_count) p->n_count = k->rest;
+        if (k->part_bytes() > split) split = k->part_bytes();
+    }
     p->off_count = take(p->n_count * 4);
+    p->off_split = take(split);
     p->off_x = take(xs);
     p->off_xt[0] = take(xs);
     p->off_xt[1] = take(xs);
@@ -474,8 +650,18 @@ int make_plan(const dsvc_ortho_cfg* c, Plan* p) {
 
 template <int T, bool MUON, int P>
 int prep(const dsvc_ortho_cfg* c, const Plan& p, const void* in, View iv, const MuonArgs& mu, char* ws, hipStream_t st) {
-    hipLaunchKernelGGL((k_ns_sums<T, MUON>), dim3(p.n_part, c->batch), dim3(256), 0, st, in, iv, c->rows, c->cols, mu, (double*)(ws + p.off_part),
-                       (int*)(ws + p.off_count), (int)p.n_count);
+    constexpr int VEC = T == F32 ? 4 : 8;
+    const bool flat = (c->rows == 1 || iv.ld == c->cols) && (!MUON || c->rows == 1 || mu.mv.ld == c->cols);
+    const int rows = flat ? 1 : c->rows;
+    const long long cols = flat ? (long long)c->rows * c->cols : c->cols;
+    auto fits = [&](const void* q, const View& v, int esize) {
+        return (uintptr_t)q % 16 == 0 && (rows == 1 || v.ld * esize % 16 == 0) && (c->batch == 1 || v.bs * esize % 16 == 0);
+    };
+    const bool vec = cols % VEC == 0 && fits(in, iv, T == F32 ? 4 : 2) && (!MUON || fits(mu.mom, mu.mv, 4));
+    double* part = (double*)(ws + p.off_part);
+    int* count = (int*)(ws + p.off_count);
+    if (vec) hipLaunchKernelGGL((k_ns_sums<T, MUON, VEC>), dim3(p.n_part, c->batch), dim3(256), 0, st, in, iv, rows, cols, mu, part, count, (int)p.n_count);
+    else hipLaunchKernelGGL((k_ns_sums<T, MUON, 1>), dim3(p.n_part, c->batch), dim3(256), 0, st, in, iv, rows, cols, mu, part, count, (int)p.n_count);
     hipLaunchKernelGGL((k_ns_prep<T, MUON, P>), dim3(p.np / 64, p.mp / 64, c->batch), dim3(256), 0, st, in, iv, c->rows, c->cols, p.tall, mu,
                        (const double*)(ws + p.off_part), p.n_part, (double)c->eps, (_Float16*)(ws + p.off_x), (_Float16*)(ws + p.off_xt[0]), p.mp, p.np,
                        (Scalars*)(ws + p.off_sc));
@@ -497,23 +683,23 @@ int iterate(const dsvc_ortho_cfg* c, const Plan& p, void* out, View ov, const Mu
     for (int k = 0; k < c->steps; ++k) {
         _Float16 *xt = (_Float16*)(ws + p.off_xt[k & 1]), *xt1 = (_Float16*)(ws + p.off_xt[(k + 1) & 1]);
         NsGemm g{};
-        g.batch = c->batch; g.slices = 1; g.sc = (const Scalars*)(ws + p.off_sc); g.step = k; g.dec = p.dec;
+        g.part = (float*)(ws + p.off_split); g.count = (int*)(ws + p.off_count); g.sc = (const Scalars*)(ws + p.off_sc); g.step = k; g.dec = p.dec;
         g.a = g.b = x; g.a_bs = g.b_bs = xs; g.nk16 = p.np / 16;
         g.ot = a; g.ot_bs = as; g.ot_nk16 = p.mp / 16;
         g.c2 = A_SCALE / (X_SCALE * X_SCALE);
-        DSVC_TRY((gemm<P, GRAM>(g, p.mp, p.mp, st)));
+        DSVC_TRY((gemm<P, GRAM>(g, p.gram, st)));
         g.a = g.b = a; g.a_bs = g.b_bs = as; g.nk16 = p.mp / 16;
         g.ot = m; g.am = a;
         g.c0 = c->coef[0] * A_SCALE; g.c1 = c->coef[1]; g.c2 = c->coef[2] / A_SCALE;
-        DSVC_TRY((gemm<P, POLY>(g, p.mp, p.mp, st)));
+        DSVC_TRY((gemm<P, POLY>(g, p.poly, st)));
         g.a = m; g.b = xt; g.b_bs = xs;
         g.o = x; g.o_bs = xs; g.o_nk16 = p.np / 16;
         g.ot = xt1; g.ot_bs = xs;
         g.c2 = 1.f / A_SCALE;
-        if (k + 1 < c->steps) { DSVC_TRY((gemm<P, FULL>(g, p.mp, p.np, st))); continue; }
+        if (k + 1 < c->steps) { DSVC_TRY((gemm<P, FULL>(g, p.full, st))); continue; }
         g.c2 = c->scale / (A_SCALE * X_SCALE);
         g.out = out; g.ov = ov; g.dtype = c->dtype; g.m = p.m; g.n = p.n; g.tall = p.tall; g.mu = mu;
-        DSVC_TRY((gemm<P, FINAL>(g, p.mp, p.np, st)));
+        DSVC_TRY((gemm<P, FINAL>(g, p.full, st)));
     }
     return DSVC_OK;
 }
