@@ -151,6 +151,9 @@ SYMBOLS = [
                                                ctypes.POINTER(ctypes.c_int64)]),
     ("dsvc_trainer_bind", ctypes.c_int, [_VP, _VP, _VP]),
     ("dsvc_trainer_set_schedule", ctypes.c_int, [_VP, _VP, _VP, ctypes.c_int32, _VP, _VP, ctypes.c_int32]),
+    ("dsvc_trainer_set_cond_grad", ctypes.c_int, [_VP, _VP, ctypes.c_int64]),
+    ("dsvc_adamw_step_strided", ctypes.c_int, [_VP, _VP, _VP, _VP, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_float, ctypes.c_float, ctypes.c_float,
+                                               ctypes.c_float, ctypes.c_float, ctypes.c_int64, _VP, ctypes.c_float, _VP]),
     ("dsvc_trainer_step", ctypes.c_int, [_VP, ctypes.POINTER(TrainArgs), _VP, _VP]),
     ("dsvc_trainer_step_begin", ctypes.c_int, [_VP, ctypes.POINTER(TrainArgs), _VP]),
     ("dsvc_trainer_check", ctypes.c_int, [_VP, _VP]),

@@ -8,14 +8,17 @@ hparams) -- no device log/pow decides a bin and nothing leaves the device.  The 
 Registered under the attribute name ``fs2`` so a reference checkpoint's ``fs2.*`` keys load strictly; the
 parameters the disabled FastSpeech2 branches own (mel_out, pitch_predictor) are accepted and kept as buffers.
 
-``use_energy_embed`` (fs2.py:81-82,143-144,240-247; round 4): decoder_inp additionally gets energy_embed[clamp(energy * 256 // 4, max=255)]
-before the mask -- an exact embedding lookup, done with torch ops behind the device builder (both shipped configs leave it off).  The
+``use_energy_embed`` (fs2.py:81-82,143-144,240-247): decoder_inp additionally gets energy_embed[clamp(energy * 256 // 4, max=255)] before the
+mask -- an exact embedding lookup behind the device builder (tokens.TokenEmbeddingHip; both shipped configs leave it off).  Its table trains: with
+``infer=False`` decoder_inp carries the autograd graph of that lookup.  The
 speaker branches (``use_spk_id`` / ``use_spk_embed``) stay rejected: the reference's own constructor has ``spk_embed_proj`` commented out
 (fs2.py:32-39, "not used"), so its forward raises AttributeError on them and no checkpoint of this architecture carries such a table."""
 import numpy as np
 import torch
 from torch import nn
 import torch.nn.functional as F
+
+from .tokens import TokenEmbeddingHip
 
 
 def f0_to_coarse(f0, hp):
@@ -84,7 +87,7 @@ class CondBuilder(nn.Module):
         nn.init.normal_(self.pitch_embed.weight, mean=0, std=self.hidden_size ** -0.5)
         nn.init.constant_(self.pitch_embed.weight[self.padding_idx], 0)
         if hparams.get("use_energy_embed"):                       # fs2.py:81-82
-            self.energy_embed = nn.Embedding(256, self.hidden_size, self.padding_idx)
+            self.energy_embed = TokenEmbeddingHip(256, self.hidden_size, self.padding_idx)
             nn.init.normal_(self.energy_embed.weight, mean=0, std=self.hidden_size ** -0.5)
             nn.init.constant_(self.energy_embed.weight[self.padding_idx], 0)
         self._extras = {}          # checkpointed-but-unused fs2.* tensors (mel_out, pitch_predictor, ...)
@@ -109,7 +112,10 @@ class CondBuilder(nn.Module):
 
     def check_alignment(self):
         """Raise IndexError if any device-path call since the last check was given a mel2ph entry outside [0, number of content units] -- what
-        torch.gather raises immediately in the reference (fs2.py:100-102); here such frames silently got zero content.  Synchronises."""
+        torch.gather raises immediately in the reference (fs2.py:100-102); here such frames silently got zero content.  The same for frame energies
+        below zero, which have no row in the energy table.  Synchronises."""
+        if hasattr(self, "energy_embed"):
+            self.energy_embed.check()
         if self._oob is not None:
             bad, self._oob = bool(self._oob.item()), None
             if bad:
@@ -190,6 +196,11 @@ class CondBuilder(nn.Module):
             coarse[b, :n] = f0_to_coarse(d.clone(), hp)[0]
         return f0_denorm, coarse
 
+    @staticmethod
+    def energy_tokens(energy):
+        """Row of the energy table of every frame (fs2.py:240-247)."""
+        return torch.clamp(energy * 256 // 4, max=255).long()
+
     def forward(self, hubert, mel2ph=None, spk_embed=None, ref_mels=None, f0=None, uv=None, energy=None,
                 skip_decoder=True, spk_embed_dur_id=None, spk_embed_f0_id=None, infer=False, **kwargs):
         hp = self.hp
@@ -204,17 +215,20 @@ class CondBuilder(nn.Module):
             if energy is None:
                 raise ValueError("use_energy_embed: forward() needs the frame energies (the reference indexes None here)")
             ret["energy_pred"] = energy
-            e_idx = torch.clamp(energy.to(hubert.device) * 256 // 4, max=255).long()
+            e_idx = self.energy_tokens(energy.to(hubert.device))
             e_emb = self.energy_embed(e_idx)
         dev = hubert.device
         if hp.get("pitch_norm", "log") != "log":
             raise NotImplementedError("pitch_norm must be 'log'")
         if hubert.is_cuda:
-            # NOT differentiable: the tensors below carry no autograd graph even with grad enabled (the drop-ins are inference modules; the
-            # training branch, GaussianDiffusionHip.forward(infer=False), gets d pitch_embed from dsvc_trainer_step, not from a graph over this)
+            # NOT differentiable but for the energy table: the tensors below carry no other autograd graph even with grad enabled (the drop-ins are
+            # inference modules; the training branch, GaussianDiffusionHip.forward(infer=False), gets d pitch_embed from dsvc_trainer_step, not from a
+            # graph over this, and hands d loss / d decoder_inp to the energy table's lookup)
             dec, cond, f0_denorm, coarse = self._build_device(hubert, mel2ph, f0, uv)
             if e_emb is not None:                                             # (x + e) * mask = x * mask + e * mask: the mask is 0 / 1
-                dec = dec + e_emb.detach() * (mel2ph > 0).to(dec.dtype)[:, :, None]
+                if infer:
+                    e_emb = e_emb.detach()
+                dec = dec + e_emb * (mel2ph > 0).to(dec.dtype)[:, :, None]
                 cond = dec.transpose(1, 2).contiguous()
             ret.update(f0_denorm=f0_denorm, pitch_pred=coarse.unsqueeze(-1), decoder_inp=dec, cond_bht=cond)
             return ret

@@ -309,6 +309,37 @@ struct TEpiDxT {
     }
 };
 
+// d loss / d cond of one layer, W_c^T dy, added to the frames' rows [clip * T + t][H] (first: stored); the loss scale leaves on the way
+struct TEpiCondBwdT {
+    struct Args { float* out; int H, T, first; float unscale; RowInfo ri; };
+    template <int NT_N>
+    __device__ __forceinline__ void init(const Args&, int, int, int, f32x16 (&acc)[NT_N]) const {
+#pragma unroll
+        for (int nt = 0; nt < NT_N; ++nt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[nt][i] = 0.f;
+    }
+    template <int NT_N>
+    __device__ __forceinline__ void finish(const Args& e, int mt, int row0, int lane, f32x16 (&acc)[NT_N]) const {
+        const int cb = mt * 32 + 16 * (lane >> 5);
+        if (cb >= e.H) return;
+#pragma unroll
+        for (int nt = 0; nt < NT_N; ++nt) {
+            const int frame = row0 + 32 * nt + (lane & 31);
+            if (!e.ri.valid(frame)) continue;
+            const int clip = frame / e.ri.clip_stride, t = frame - clip * e.ri.clip_stride;
+            float* p = e.out + ((size_t)clip * e.T + t) * e.H + cb;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                f32x4 v = e.first ? f32x4{0.f, 0.f, 0.f, 0.f} : ld4(p + 4 * q);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] += acc[nt][4 * q + i] * e.unscale;
+                st4(p + 4 * q, v);
+            }
+        }
+    }
+};
+
 // fp32 rows [rows][ld_src] (+ add[clip]) -> fp16 [hi | lo] row planes [rows][2 Cp]: the tgemm operand of layer 0 and of the conditioner
 // projection; invalid rows and the channel padding are written as zeros
 __global__ void k_rows_to_planes(const float* __restrict__ src, int ld_src, int C, const float* __restrict__ add, int add_stride,
@@ -780,9 +811,8 @@ __global__ void k_iota(int* p, int base, int n) {
 }
 
 // AdamW (torch.optim.AdamW semantics: decoupled weight decay, bias-corrected moments), gradients pre-scaled by gscale
-__global__ void k_adamw(float* __restrict__ p, const float* __restrict__ g, float* __restrict__ m, float* __restrict__ v, size_t n,
-                        float lr, float b1, float b2, float eps, float wd, float bc1, float bc2, const float* __restrict__ gscale_dev, float gscale) {
-    const float gs = gscale_dev ? *gscale_dev : gscale;
+__device__ __forceinline__ void adamw(float* __restrict__ p, const float* __restrict__ g, float* __restrict__ m, float* __restrict__ v, size_t n,
+                                      float lr, float b1, float b2, float eps, float wd, float bc1, float bc2, float gs) {
     for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (size_t)gridDim.x * blockDim.x) {
         const float gr = g[i] * gs;
         float w = p[i];
@@ -794,6 +824,16 @@ __global__ void k_adamw(float* __restrict__ p, const float* __restrict__ g, floa
         w -= (lr / bc1) * mi / denom;
         p[i] = w;
     }
+}
+__global__ void k_adamw(float* __restrict__ p, const float* __restrict__ g, float* __restrict__ m, float* __restrict__ v, size_t n,
+                        float lr, float b1, float b2, float eps, float wd, float bc1, float bc2, const float* __restrict__ gscale_dev, float gscale) {
+    adamw(p, g, m, v, n, lr, b1, b2, eps, wd, bc1, bc2, gscale_dev ? *gscale_dev : gscale);
+}
+// the same for parts of n floats, `stride` apart (one tensor of every residual layer): blockIdx.y = part
+__global__ void k_adamw_strided(float* __restrict__ p, const float* __restrict__ g, float* __restrict__ m, float* __restrict__ v, size_t n, size_t stride,
+                                float lr, float b1, float b2, float eps, float wd, float bc1, float bc2, const float* __restrict__ gscale_dev, float gscale) {
+    const size_t o = blockIdx.y * stride;
+    adamw(p + o, g + o, m + o, v + o, n, lr, b1, b2, eps, wd, bc1, bc2, gscale_dev ? *gscale_dev : gscale);
 }
 
 __global__ void k_sqsum(const float* __restrict__ g, size_t n, float* __restrict__ out) {
@@ -871,6 +911,11 @@ struct dsvc_trainer {
     DevBuf dOh, dyh;                               // planes of dO [rows][2 C2p] and of dy [TGUARD + rows + TGUARD][2 C2p]
     DevBuf oT_t, dT_t;                             // W_o^T and the flipped W_d^T, rows = input channels of the layer
     size_t oT_halfs = 0, dT_halfs = 0;
+    // d loss / d cond (dsvc_trainer_set_cond_grad): W_c^T of every layer, packed only while it is asked for
+    float* cond_grad = nullptr;
+    int64_t cond_grad_rows = 0;
+    DevBuf cT_t, t_cond_rm;
+    size_t cT_halfs = 0;
     // round 5: the residual layers' weight gradients are contracted straight from these frame-major planes (wgrad.h: wgrad_fm_kernel) instead of
     // channel-major copies a k_split_t pass writes -- which needs layer l's x / g planes alive in the backward pass: every layer gets its own
     // (2 x 270 MB at the 64 x 128 batch).  fm = the architecture fits the kernel's tiles (C % 128, H % 128: the shipped configs; others keep k_split_t)
@@ -896,7 +941,7 @@ struct dsvc_trainer {
         for (DevBuf* b : {&sa, &sb, &spec_min, &spec_max, &xt, &xs, &sig, &tau, &g, &skip, &ypre, &s2pre, &eps, &deps, &condT, &tstep,
                           &clipid, &iotaB, &e0, &e1pre, &e1, &e2, &filmB, &dfilm, &de2, &de1, &de1pre, &dx, &dxin, &dO, &dy, &ds2pre,
                           &dh0, &loss, &AT, &BT, &wpart, &pack_dev, &bin_count, &bin_cursor, &bin_segs, &bin_nsegs, &bin_order, &bin_S,
-                          &xhP, &ghP, &condHP, &gate_t, &out_t, &cproj_t, &t_gate_rm, &t_gate_rs, &t_out_rm, &tpack_dev, &dOh, &dyh, &oT_t, &dT_t, &wbias})
+                          &xhP, &ghP, &condHP, &gate_t, &out_t, &cproj_t, &t_gate_rm, &t_gate_rs, &t_out_rm, &tpack_dev, &dOh, &dyh, &oT_t, &dT_t, &wbias, &cT_t, &t_cond_rm})
             b->release();
         if (step_err) (void)hipHostFree(step_err);
         auto rel = [](Packed& p) { p.w.release(); };
@@ -1033,6 +1078,10 @@ int dsvc_trainer::repack(hipStream_t st) {
         // W_o^T(c, k) = W_o[k][c]
         tpack_q.push_back(TPackDesc{P(q + "output_projection.weight"), t_out_rm.as<int>(), nullptr, oT_t.as<_Float16>() + (size_t)l * oT_halfs, 2 * C, 1, C2p, C / 32, 1, C, 1, 0});
         // transposed conv: dxin[c] = sum_tap sum_o W_d[o][c][2 - tap] * dy[row + (tap-1)*d][o]
+        // dcond[h] += sum_o W_c[o][h] dy[o]
+        if (cond_grad)
+            tpack_q.push_back(TPackDesc{P(q + "conditioner_projection.weight"), t_cond_rm.as<int>(), nullptr, cT_t.as<_Float16>() + (size_t)l * cT_halfs, 2 * C, 1, C2p,
+                                        ceil_div(H, 32), 1, H, 1, 0});
         tpack_q.push_back(TPackDesc{P(q + "dilated_conv.weight"), t_out_rm.as<int>(), nullptr, dT_t.as<_Float16>() + (size_t)l * dT_halfs, 2 * C, 3, C2p, C / 32, 3, (long long)C * 3, 1, 1});
     }
     return flush_packs(st);
@@ -1274,6 +1323,22 @@ int dsvc_trainer::run(int phases, int l_hi, int l_lo, const dsvc_train_args* ta_
     if ((phases & PH_END) && !(phases & PH_LAYERS) && next_layer != 0) return fail(DSVC_ESTATE, "trainer: %d residual layers still to go", next_layer);
     if (phases & PH_BEGIN) {
         DSVC_TRY(ensure_ws(B, T, st));
+        if (cond_grad) {
+            if ((int64_t)B * T > cond_grad_rows) return fail(DSVC_EINVAL, "trainer: %d x %d frames, the gradient of cond has %lld rows", B, T, (long long)cond_grad_rows);
+            const int tiles = ceil_div(H, 32);
+            cT_halfs = tpacked_halfs(tiles, 1, C2p, 2, 1);
+            DSVC_TRY(cT_t.alloc(cT_halfs * L * 2));
+            if (!t_cond_rm.p) {
+                std::vector<int> rm(tiles * 32);
+                for (int q = 0; q < tiles * 32; ++q) {
+                    const int h = (q >> 5) * 32 + trow_to_ch16(q & 31);
+                    rm[q] = h < H ? h : -1;
+                }
+                DSVC_TRY(t_cond_rm.alloc(rm.size() * 4));
+                DSVC_HIP(hipMemcpyAsync(t_cond_rm.p, rm.data(), rm.size() * 4, hipMemcpyHostToDevice, st));
+                DSVC_HIP(hipStreamSynchronize(st));
+            }
+        }
         DSVC_TRY(repack(st));
     }
     const RowInfo ri{Tp, T, nr};
@@ -1446,6 +1511,14 @@ int dsvc_trainer::run(int phases, int l_hi, int l_lo, const dsvc_train_args* ta_
                                  dyh.as<_Float16>() + (size_t)TGUARD * 2 * C2p, C, C2p, ri};
             DSVC_TRY((tg<TEpiGateBwdT, 1>(dOh.as<_Float16>(), C2p, 1, 1, oT_t.as<_Float16>() + (size_t)l * oT_halfs, C / 32, e, st, C2p % 256 == 0 ? 256 : 128)));
         }
+        if (cond_grad) {   // (tiles of 32 frames: H = 256 is one pass of eight waves)
+            TGemmArgs a{};
+            a.kp_cin = C2p % 256 == 0 ? 256 : 128;
+            a.x = dyh.as<_Float16>() + (size_t)TGUARD * 2 * C2p; a.cin = C2p; a.taps = 1; a.dil = 1; a.w = cT_t.as<_Float16>() + (size_t)l * cT_halfs;
+            a.m_tiles = ceil_div(H, 32); a.w_planes = 2; a.n_variants = 1;
+            const TEpiCondBwdT::Args e{cond_grad, H, T, l == L - 1, unscale, ri};
+            DSVC_TRY((tgemm_launch<1, 8, 2, 4, 2, TEpiCondBwdT, 1, 1, 2, 0, 1>(a, e, rows, ceil_div(a.m_tiles, 8), st)));
+        }
         // dW_d[o][c][tap] = sum_n dy[n][o] (x^l + film)[n + (tap-1) d][c]  and  dW_c[o][h] = sum_n dy[n][o] cond[n][h]  share dy^T: ONE
         // contraction over the k axis [tap 0 | tap 1 | tap 2 | cond]
         WgradSegs sg{};
@@ -1616,6 +1689,14 @@ int dsvc_trainer_set_schedule(dsvc_trainer* t, const float* sqrt_ac, const float
     return DSVC_OK;
 }
 
+int dsvc_trainer_set_cond_grad(dsvc_trainer* t, float* cond_grad, int64_t rows) {
+    if (!t || (cond_grad && rows < 1)) return fail(DSVC_EINVAL, "bad argument");
+    if (t->next_layer >= 0) return fail(DSVC_ESTATE, "trainer: a step is in flight");
+    t->cond_grad = cond_grad;
+    t->cond_grad_rows = cond_grad ? rows : 0;
+    return DSVC_OK;
+}
+
 int dsvc_trainer_check(dsvc_trainer* t, void* stream) {
     if (!t) return fail(DSVC_EINVAL, "null handle");
     DSVC_HIP(hipStreamSynchronize((hipStream_t)stream));
@@ -1668,6 +1749,18 @@ int dsvc_adamw_step(float* params, const float* grads, float* exp_avg, float* ex
     const int blocks = (int)((n + 255) / 256 < 8192 ? (n + 255) / 256 : 8192);
     hipLaunchKernelGGL(k_adamw, dim3(blocks > 0 ? blocks : 1), dim3(256), 0, (hipStream_t)stream, params, grads, exp_avg, exp_avg_sq, (size_t)n, lr, beta1,
                        beta2, eps, weight_decay, bc1, bc2, grad_scale_dev, grad_scale);
+    DSVC_HIP(hipGetLastError());
+    return DSVC_OK;
+}
+
+int dsvc_adamw_step_strided(float* params, const float* grads, float* exp_avg, float* exp_avg_sq, int64_t n, int64_t parts, int64_t stride, float lr, float beta1,
+                            float beta2, float eps, float weight_decay, int64_t step, const float* grad_scale_dev, float grad_scale, void* stream) {
+    if (!params || !grads || !exp_avg || !exp_avg_sq || n < 0 || parts < 0 || parts > 65535 || step < 1 || (parts > 1 && stride < n)) return fail(DSVC_EINVAL, "bad argument");
+    if (!n || !parts) return DSVC_OK;
+    const float bc1 = 1.0f - powf(beta1, (float)step), bc2 = 1.0f - powf(beta2, (float)step);
+    const int blocks = (int)((n + 255) / 256 < 8192 ? (n + 255) / 256 : 8192);
+    hipLaunchKernelGGL(k_adamw_strided, dim3(blocks, (unsigned)parts), dim3(256), 0, (hipStream_t)stream, params, grads, exp_avg, exp_avg_sq, (size_t)n, (size_t)stride, lr,
+                       beta1, beta2, eps, weight_decay, bc1, bc2, grad_scale_dev, grad_scale);
     DSVC_HIP(hipGetLastError());
     return DSVC_OK;
 }

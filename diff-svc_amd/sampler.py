@@ -48,11 +48,13 @@ class _DiffLoss(torch.autograd.Function):
     for torch.optim and clip_grad_norm_, which treat every ``.grad`` independently; clone before mutating one ``.grad`` through another's base."""
 
     @staticmethod
-    def forward(ctx, owner, step_args, *params):
+    def forward(ctx, owner, step_args, decoder_inp, *params):
         h, flat_p, flat_g = owner._trainer(params[0].device)
         with torch.no_grad():                            # one fused multi-tensor copy instead of 172 launches
             torch._foreach_copy_([flat_p[off:off + n].view(p.shape) for (name, off, n), p in zip(h.layout, params)], [p.detach() for p in params])
-        loss = h.step(*step_args[:3], pitch=step_args[3], mel2ph=step_args[4], seed=step_args[5])
+        mels, t, pitch, mel2ph, seed = step_args
+        ctx.cond_grad = torch.empty_like(decoder_inp, memory_format=torch.contiguous_format) if ctx.needs_input_grad[2] else None
+        loss = h.step(mels, decoder_inp.detach().transpose(1, 2).contiguous(), t, pitch=pitch, mel2ph=mel2ph, seed=seed, cond_grad=ctx.cond_grad)
         ctx.layout, ctx.shapes = h.layout, [p.shape for p in params]
         ctx.grads = flat_g.clone()                       # the flat gradient buffer is overwritten by the next forward
         return loss.reshape(()).clone()
@@ -60,7 +62,7 @@ class _DiffLoss(torch.autograd.Function):
     @staticmethod
     def backward(ctx, g):
         scaled = ctx.grads * g
-        return (None, None) + tuple(scaled[off:off + n].view(shape) for (name, off, n), shape in zip(ctx.layout, ctx.shapes))
+        return (None, None, None if ctx.cond_grad is None else ctx.cond_grad * g) + tuple(scaled[off:off + n].view(shape) for (name, off, n), shape in zip(ctx.layout, ctx.shapes))
 
 
 class GaussianDiffusionHip(nn.Module):
@@ -135,9 +137,8 @@ class GaussianDiffusionHip(nn.Module):
             named = dict(self.named_parameters())
             self._train_params = (h, [named[name] for name, _, _ in h.layout])
         params = self._train_params[1]
-        cond = ret["decoder_inp"].detach().transpose(1, 2).contiguous()
         pitch = ret["pitch_pred"].detach().squeeze(-1) if "pitch_pred" in ret else None
-        return _DiffLoss.apply(self, (ref_mels.detach(), cond, t, pitch, mel2ph, seed), *params)
+        return _DiffLoss.apply(self, (ref_mels.detach(), t, pitch, mel2ph, seed), ret["decoder_inp"], *params)
 
     def _handle(self, use="ddpm", speedup=1, frames=None, clips=None):
         den = self.denoise_fn.handle(use, speedup, frames, clips)
@@ -156,9 +157,8 @@ class GaussianDiffusionHip(nn.Module):
     def forward(self, hubert, mel2ph=None, spk_embed=None, ref_mels=None, f0=None, uv=None, energy=None, infer=False,
                 **kwargs):
         if not infer:      # training branch: the pitch embedding's gradient comes from dsvc_trainer_step, not from an autograd graph over fs2
-            if self.hp.get("use_energy_embed"):
-                raise NotImplementedError("training with use_energy_embed: dsvc_trainer_step produces no gradient for fs2.energy_embed.weight")
-            with torch.no_grad():
+            # (only the energy table, where there is one, keeps a graph: the loss's backward pass ends in d loss / d decoder_inp)
+            with torch.set_grad_enabled(torch.is_grad_enabled() and bool(self.hp.get("use_energy_embed"))):
                 ret = self.fs2(hubert, mel2ph, spk_embed, None, f0, uv, energy, skip_decoder=True, infer=False)
             ret.pop("cond_bht", None)
             ret["diff_loss"] = self._p_losses(ret, ref_mels, mel2ph, t=kwargs.get("t"), seed=kwargs.get("seed"))

@@ -18,6 +18,8 @@ import torch
 from . import _lib
 from ._lib import check, lib, ptr, stream_ptr
 from .cond import CondBuilder
+from .muon import muon_step_, rms_scale
+from .tokens import embed_tokens_grad
 
 
 class TrainerHandle:
@@ -25,6 +27,7 @@ class TrainerHandle:
         self._h = ctypes.c_void_p(0)
         self._L = lib()                                    # the library this handle lives in (product, or the test-hooks build: _lib.hooks_build)
         self._inflight = None                              # tensors of the step between step_begin() and step_end()
+        self._cond_grad = None                             # where the step in flight writes d loss / d cond
         self.cfg = _lib.TrainerCfg(hp["audio_num_mel_bins"], hp["hidden_size"], hp["residual_channels"], hp["residual_layers"],
                                    hp["dilation_cycle_length"], int(hp.get("timesteps", 1000)), 1 if loss_type == "l1" else 0, pitch_vocab)
         self._ck(self._L.dsvc_trainer_create(ctypes.byref(self.cfg), ctypes.byref(self._h)))
@@ -76,15 +79,29 @@ class TrainerHandle:
                            clip_ids.data_ptr() if clip_ids is not None else None)
         return a, (mel, cond, t, pitch, mel2ph, clip_ids)            # the tensors stay referenced while the step is enqueued
 
-    def step(self, mel, cond, t, pitch=None, mel2ph=None, seed=0, first_clip=0, clip_ids=None, loss_out=None):
+    def _want_cond_grad(self, g, mel=None):
+        if g is None and self._cond_grad is None:
+            return
+        if g is not None and (g.dtype != torch.float32 or not g.is_cuda or not g.is_contiguous() or tuple(g.shape) != (*mel.shape[:2], self.cfg.hidden)):
+            raise ValueError("cond_grad must be float32 [%d, %d, %d] on the HIP device" % (*mel.shape[:2], self.cfg.hidden))
+        self._ck(self._L.dsvc_trainer_set_cond_grad(self._h, None if g is None else g.data_ptr(), 0 if g is None else g.shape[0] * g.shape[1]))
+        self._cond_grad = g
+
+    def step(self, mel, cond, t, pitch=None, mel2ph=None, seed=0, first_clip=0, clip_ids=None, loss_out=None, cond_grad=None):
+        """cond_grad: a float32 [B, T, H] tensor that gets d loss / d cond, transposed (None: not computed)."""
         a, keep = self._args(mel, cond, t, pitch, mel2ph, seed, first_clip, clip_ids)
         loss = loss_out if loss_out is not None else torch.empty(1, device=mel.device, dtype=torch.float32)
-        self._ck(self._L.dsvc_trainer_step(self._h, ctypes.byref(a), ptr(loss), stream_ptr()))
+        self._want_cond_grad(cond_grad, mel)
+        try:
+            self._ck(self._L.dsvc_trainer_step(self._h, ctypes.byref(a), ptr(loss), stream_ptr()))
+        finally:
+            self._want_cond_grad(None)
         return loss
 
     # the same step in phases (include/dsvc.h): after each call a contiguous slice of the gradient buffer is final
-    def step_begin(self, mel, cond, t, pitch=None, mel2ph=None, seed=0, first_clip=0, clip_ids=None):
+    def step_begin(self, mel, cond, t, pitch=None, mel2ph=None, seed=0, first_clip=0, clip_ids=None, cond_grad=None):
         a, self._inflight = self._args(mel, cond, t, pitch, mel2ph, seed, first_clip, clip_ids)
+        self._want_cond_grad(cond_grad, mel)
         self._ck(self._L.dsvc_trainer_step_begin(self._h, ctypes.byref(a), stream_ptr()))
 
     def step_layers(self, l_hi, l_lo):
@@ -96,6 +113,7 @@ class TrainerHandle:
         loss = loss_out if loss_out is not None else torch.empty(1, device=self._inflight[0].device, dtype=torch.float32)
         self._ck(self._L.dsvc_trainer_step_end(self._h, ptr(loss), stream_ptr()))
         self._inflight = None
+        self._want_cond_grad(None)
         return loss
 
     def __del__(self):
@@ -138,9 +156,45 @@ def allreduce_mean_(flat, group=None):
     return flat
 
 
+ENERGY = "fs2.energy_embed.weight"
+
+
+def muon_groups(layout, shapes):
+    """What ``matrix_optimizer: muon`` does with each tensor of the flat layout: ([(offset, batch, stride, rows, cols)], [(offset, numel, parts, stride)]).
+    The first list holds the inner matrices -- the residual layers' convolutions and projections, one group of all layers each, the step-embedding MLP
+    and the skip projection; a convolution [out, in, k] is the matrix [out, in k] -- and is orthogonalised.  The second holds everything else for
+    AdamW: the first and last projection, biases and embedding tables, neighbours in one piece, a layer's tensor as parts of all layers."""
+    inner = lambda n: n.endswith(".weight") and (".residual_layers." in n or ".mlp." in n or ".skip_projection." in n)
+    layer = lambda n: int(n.split(".residual_layers.")[1].split(".")[0]) if ".residual_layers." in n else None
+    per_layer, muon, adam = {}, [], []
+    for name, off, numel in layout:
+        if layer(name) is not None:
+            per_layer.setdefault(name.split(".", 3)[3], []).append((off, numel, name))
+        elif inner(name):
+            muon.append((off, 1, 0, shapes[name][0], numel // shapes[name][0]))
+        elif adam and adam[-1][2] == 1 and adam[-1][0] + adam[-1][1] == off:
+            adam[-1] = (adam[-1][0], adam[-1][1] + numel, 1, 0)
+        else:
+            adam.append((off, numel, 1, 0))
+    for parts in per_layer.values():
+        off, numel, name = parts[0]
+        stride = parts[1][0] - off if len(parts) > 1 else 0
+        assert all(p[0] == off + i * stride and p[1] == numel for i, p in enumerate(parts)), name
+        if inner(name):
+            muon.append((off, len(parts), stride, shapes[name][0], numel // shapes[name][0]))
+        else:
+            adam.append((off, numel, len(parts), stride))
+    return muon, adam
+
+
 class DiffusionTrainerHip:
     """state: a GaussianDiffusion state dict (no ``model.`` prefix).  hp keys read beyond the architecture: ``diff_loss_type``,
-    ``lr``, ``optimizer_adam_beta1/2``, ``weight_decay``, ``clip_grad_norm``, ``decay_steps`` (training/config_nsf.yaml)."""
+    ``lr``, ``optimizer_adam_beta1/2``, ``weight_decay``, ``clip_grad_norm``, ``decay_steps`` (training/config_nsf.yaml).
+
+    ``use_energy_embed`` (fs2.py:81-82): the energy table trains too -- its gradient is d loss / d cond, which the step leaves behind, added up by
+    token (tokens.embed_tokens_grad); the steps then take the frames' ``energy``.
+    ``matrix_optimizer: muon``: the inner matrices (muon_groups) take orthogonalised momentum steps (muon.muon_step_) of the root mean square of AdamW's, the
+    rest stays on AdamW; keys ``muon_lr`` (default: ``lr``), ``muon_momentum`` (0.95), ``muon_steps`` (5), ``muon_precision`` (None, "f16", "f16_x3")."""
 
     def __init__(self, hp, state, device="cuda", group=None):
         if not torch.cuda.is_available():
@@ -148,33 +202,44 @@ class DiffusionTrainerHip:
         self.hp, self.group, self.device = hp, group, device
         self.h = TrainerHandle(hp, hp.get("diff_loss_type", "l2"), state["fs2.pitch_embed.weight"].shape[0])
         n = self.h.n_floats
+        self.layout = list(self.h.layout)
+        self.energy_vocab = state[ENERGY].shape[0] if hp.get("use_energy_embed") else 0
+        if self.energy_vocab:                              # behind the handle's tensors in the same flat buffers
+            self.layout.append((ENERGY, n, state[ENERGY].numel()))
+            n += state[ENERGY].numel()
+        self.n_floats = n
+        if hp.get("matrix_optimizer", "adamw") not in ("adamw", "muon"):
+            raise ValueError("matrix_optimizer must be 'adamw' or 'muon', got %r" % (hp["matrix_optimizer"],))
         self.params = torch.zeros(n, device=device, dtype=torch.float32)
         self.grads = torch.zeros(n, device=device, dtype=torch.float32)
         self.exp_avg = torch.zeros(n, device=device, dtype=torch.float32)
         self.exp_avg_sq = torch.zeros(n, device=device, dtype=torch.float32)
         self._aux = torch.zeros(4, device=device, dtype=torch.float32)          # [0] ||g||^2, [1] clip coefficient
         self.shapes = {}
-        for name, off, numel in self.h.layout:
+        for name, off, numel in self.layout:
             v = state[name]
             assert v.numel() == numel, (name, tuple(v.shape), numel)
             self.params[off:off + numel].copy_(v.reshape(-1).float())
             self.shapes[name] = tuple(v.shape)
         self.other = {k: v.clone() for k, v in state.items() if k not in self.shapes}     # buffers + the fs2.* tensors no gradient reaches
-        self.h.bind(self.params, self.grads)
+        self.h.bind(self.params[:self.h.n_floats], self.grads[:self.h.n_floats])
         self.h.set_schedule(state["sqrt_alphas_cumprod"], state["sqrt_one_minus_alphas_cumprod"], state["spec_min"], state["spec_max"])
         self.fs2 = CondBuilder(hp).to(device)
         off, numel = next((o, m) for nme, o, m in self.h.layout if nme == "fs2.pitch_embed.weight")
         self.fs2.pitch_embed.weight.data = self.params[off:off + numel].view(self.shapes["fs2.pitch_embed.weight"])   # shares the flat storage
+        if self.energy_vocab:
+            self.fs2.energy_embed.weight.data = self.view(self.params, ENERGY)
+        self._muon = muon_groups(self.layout, self.shapes) if hp.get("matrix_optimizer") == "muon" else None
         self.global_step = 0
         self.lr0 = float(hp.get("lr", 0.0004))
 
     def view(self, flat, name):
-        off, numel = next((o, m) for nme, o, m in self.h.layout if nme == name)
+        off, numel = next((o, m) for nme, o, m in self.layout if nme == name)
         return flat[off:off + numel].view(self.shapes[name])
 
     def state_dict(self):
         sd = {k: v.clone() for k, v in self.other.items()}
-        for name, off, numel in self.h.layout:
+        for name, off, numel in self.layout:
             sd[name] = self.params[off:off + numel].view(self.shapes[name]).detach().clone().cpu()
         return sd
 
@@ -186,29 +251,46 @@ class DiffusionTrainerHip:
         return self.lr0 * 0.5 ** (max(self.global_step - 1, 0) // int(self.hp.get("decay_steps", 40000)))
 
     @torch.no_grad()
-    def forward_backward(self, hubert, mel2ph, f0, mels, t, seed=0, first_clip=0, clip_ids=None):
+    def forward_backward(self, hubert, mel2ph, f0, mels, t, seed=0, first_clip=0, clip_ids=None, energy=None):
         """loss (device scalar) of one batch; the gradients land in ``self.grads`` (this rank's, before any all-reduce)."""
-        ret = self.fs2(hubert, mel2ph, None, None, f0.clone(), None, None, infer=False)
+        ret, cond_grad = self._cond(hubert, mel2ph, f0, energy)
         cond = ret["decoder_inp"].transpose(1, 2).contiguous()
-        return self.h.step(mels, cond, t, pitch=ret["pitch_pred"].squeeze(-1), mel2ph=mel2ph, seed=seed, first_clip=first_clip, clip_ids=clip_ids)
+        loss = self.h.step(mels, cond, t, pitch=ret["pitch_pred"].squeeze(-1), mel2ph=mel2ph, seed=seed, first_clip=first_clip, clip_ids=clip_ids,
+                           cond_grad=cond_grad)
+        self._energy_grad(mel2ph, energy, cond_grad)
+        return loss
+
+    def _cond(self, hubert, mel2ph, f0, energy):
+        """The condition builder's outputs and, where the energy table trains, the tensor for d loss / d cond."""
+        ret = self.fs2(hubert, mel2ph, None, None, f0.clone(), None, energy, infer=False)
+        return ret, torch.empty_like(ret["decoder_inp"]) if self.energy_vocab else None
+
+    def _energy_grad(self, mel2ph, energy, cond_grad):
+        if cond_grad is not None:                          # padded frames reach no loss through the table: a token outside it
+            tokens = torch.where(mel2ph > 0, self.fs2.energy_tokens(energy.to(mel2ph.device)), -1)
+            embed_tokens_grad(tokens, cond_grad, self.energy_vocab, padding_idx=self.fs2.padding_idx, out=self.view(self.grads, ENERGY))
 
     @torch.no_grad()
-    def forward_backward_overlapped(self, hubert, mel2ph, f0, mels, t, seed=0, first_clip=0, clip_ids=None, layers_per_bucket=5):
+    def forward_backward_overlapped(self, hubert, mel2ph, f0, mels, t, seed=0, first_clip=0, clip_ids=None, layers_per_bucket=5, energy=None):
         """forward_backward + the gradient all-reduce (mean), bucket by bucket under the backward pass: every bucket's all-reduce is
         launched asynchronously (RCCL's own stream, ordered after the kernels that made the slice final) and waited for at the end.
         ``self.grads`` holds the averaged gradients on return."""
         import torch.distributed as dist
-        ret = self.fs2(hubert, mel2ph, None, None, f0.clone(), None, None, infer=False)
+        ret, cond_grad = self._cond(hubert, mel2ph, f0, energy)
         cond = ret["decoder_inp"].transpose(1, 2).contiguous()
         world = dist.get_world_size(self.group)
         works, loss = [], None
         for phase, hi, lo, slices in gradient_buckets(self.h.layout, int(self.hp["residual_layers"]), layers_per_bucket):
             if phase == "begin":
-                self.h.step_begin(mels, cond, t, pitch=ret["pitch_pred"].squeeze(-1), mel2ph=mel2ph, seed=seed, first_clip=first_clip, clip_ids=clip_ids)
+                self.h.step_begin(mels, cond, t, pitch=ret["pitch_pred"].squeeze(-1), mel2ph=mel2ph, seed=seed, first_clip=first_clip, clip_ids=clip_ids,
+                                  cond_grad=cond_grad)
             elif phase == "layers":
                 self.h.step_layers(hi, lo)
             else:
                 loss = self.h.step_end()
+                if self.energy_vocab:                      # d loss / d cond is final with the last residual layer
+                    self._energy_grad(mel2ph, energy, cond_grad)
+                    slices = slices + [(self.h.n_floats, self.n_floats - self.h.n_floats)]
             for o, n in slices:
                 works.append(dist.all_reduce(self.grads[o:o + n], op=dist.ReduceOp.SUM, group=self.group, async_op=True))
         for w in works:
@@ -220,7 +302,7 @@ class DiffusionTrainerHip:
     CHECK_EVERY = 100              # optimiser steps between two reads of the trainer's sticky argument flag (dsvc_trainer_check synchronises)
 
     @torch.no_grad()
-    def train_step(self, hubert, mel2ph, f0, mels, t=None, seed=None, first_clip=0, clip_ids=None, overlap=None):
+    def train_step(self, hubert, mel2ph, f0, mels, t=None, seed=None, first_clip=0, clip_ids=None, overlap=None, energy=None):
         """One optimisation step: forward + backward, all-reduce (mean) of the gradients over the ranks, gradient-norm clip, AdamW.
         overlap: all-reduce bucket by bucket under the backward pass (default: whenever a process group with more than one rank is up)."""
         import torch.distributed as dist
@@ -233,29 +315,41 @@ class DiffusionTrainerHip:
         if overlap is None:
             overlap = ddp and dist.get_world_size(self.group) > 1
         if overlap and ddp:
-            loss = self.forward_backward_overlapped(hubert, mel2ph, f0, mels, t, seed=seed, first_clip=first_clip, clip_ids=clip_ids)
+            loss = self.forward_backward_overlapped(hubert, mel2ph, f0, mels, t, seed=seed, first_clip=first_clip, clip_ids=clip_ids, energy=energy)
             self.optimizer_step(reduced=True)
         else:
-            loss = self.forward_backward(hubert, mel2ph, f0, mels, t, seed=seed, first_clip=first_clip, clip_ids=clip_ids)
+            loss = self.forward_backward(hubert, mel2ph, f0, mels, t, seed=seed, first_clip=first_clip, clip_ids=clip_ids, energy=energy)
             self.optimizer_step()
         return loss
 
     @torch.no_grad()
     def optimizer_step(self, reduced=False):
         """What follows the backward pass: all-reduce (mean) of ``self.grads`` over the ranks (unless the overlapped backward pass has done
-        it already), clip_grad_norm_, AdamW at the StepLR rate."""
+        it already), clip_grad_norm_, AdamW at the StepLR rate (``matrix_optimizer: muon``: orthogonalised momentum for the inner matrices)."""
         if not reduced:
             allreduce_mean_(self.grads, self.group)
         lr = self.lr()                                       # step k (0-based) runs at lr0 * 0.5 ** (max(k - 1, 0) // decay_steps)
         self.global_step += 1
         if self.global_step % self.CHECK_EVERY == 0:
             self.h.check()                                   # the trainer's sticky "diffusion step outside the schedule" flag: one sync per 100 steps
-        hp, n = self.hp, self.h.n_floats
+        hp, n = self.hp, self.n_floats
         clip = float(hp.get("clip_grad_norm", 1.0))
         coef = None
         if clip > 0:
             check(lib().dsvc_grad_clip_coef(ptr(self.grads), n, clip, ptr(self._aux[0:1]), ptr(self._aux[1:2]), stream_ptr()))
             coef = self._aux[1:2]
-        check(lib().dsvc_adamw_step(ptr(self.params), ptr(self.grads), ptr(self.exp_avg), ptr(self.exp_avg_sq), n, lr,
-                                    float(hp.get("optimizer_adam_beta1", 0.9)), float(hp.get("optimizer_adam_beta2", 0.98)), 1e-8,
-                                    float(hp.get("weight_decay", 0.0)), self.global_step, ptr(coef), 1.0, stream_ptr()))
+        betas, wd = (float(hp.get("optimizer_adam_beta1", 0.9)), float(hp.get("optimizer_adam_beta2", 0.98))), float(hp.get("weight_decay", 0.0))
+        if self._muon is None:
+            check(lib().dsvc_adamw_step(ptr(self.params), ptr(self.grads), ptr(self.exp_avg), ptr(self.exp_avg_sq), n, lr, *betas, 1e-8, wd,
+                                        self.global_step, ptr(coef), 1.0, stream_ptr()))
+            return
+        muon, adam = self._muon
+        for off, numel, parts, stride in adam:
+            p, g, m, v = (x[off:] for x in (self.params, self.grads, self.exp_avg, self.exp_avg_sq))
+            check(lib().dsvc_adamw_step_strided(ptr(p), ptr(g), ptr(m), ptr(v), numel, parts, stride, lr, *betas, 1e-8, wd, self.global_step, ptr(coef), 1.0,
+                                                stream_ptr()))
+        rate = lr / self.lr0 * float(hp.get("muon_lr", self.lr0)) if self.lr0 else lr
+        for off, batch, stride, rows, cols in muon:            # (the momentum is exp_avg's slice; exp_avg_sq's stays zero)
+            p, g, m = (x.as_strided((batch, rows, cols), (stride, cols, 1), off) for x in (self.params, self.grads, self.exp_avg))
+            muon_step_(p, g, m, rate, momentum=float(hp.get("muon_momentum", 0.95)), weight_decay=wd, scale=rms_scale(rows, cols),
+                       steps=int(hp.get("muon_steps", 5)), precision=hp.get("muon_precision"), grad_scale=coef)

@@ -346,6 +346,10 @@ DSVC_API int dsvc_trainer_bind(dsvc_trainer* t, float* params, float* grads);   
 /* registered buffers of GaussianDiffusion the loss needs (diffusion.py:107-108,122-123), host pointers */
 DSVC_API int dsvc_trainer_set_schedule(dsvc_trainer* t, const float* sqrt_alphas_cumprod, const float* sqrt_one_minus_alphas_cumprod, int32_t K,
                               const float* spec_min, const float* spec_max, int32_t n_spec);
+/* cond_grad [rows][H] device (retained until the next call; NULL: not computed, the default): steps that follow write d loss / d cond of frame
+ * (clip b, frame t) to row b * T + t, for whatever is trained in front of the denoiser (an energy table: dsvc_embed_tokens_grad).  A step of more
+ * than `rows` frames is refused.  Final after the last residual layer (dsvc_trainer_step_layers(.., 0)). */
+DSVC_API int dsvc_trainer_set_cond_grad(dsvc_trainer* t, float* cond_grad, int64_t rows);
 /* forward + backward of one batch: grads <- d loss / d params (overwritten), *loss_out (device float, may be NULL) <- the loss */
 DSVC_API int dsvc_trainer_step(dsvc_trainer* t, const dsvc_train_args* a, float* loss_out, void* stream);
 /* The same step in three phases, for a data-parallel host that all-reduces finished gradient slices while the backward pass of the
@@ -369,6 +373,10 @@ DSVC_API int dsvc_trainer_step_end(dsvc_trainer* t, float* loss_out, void* strea
  * when that pointer is not NULL, else by grad_scale. */
 DSVC_API int dsvc_adamw_step(float* params, const float* grads, float* exp_avg, float* exp_avg_sq, int64_t n, float lr, float beta1, float beta2,
                     float eps, float weight_decay, int64_t step, const float* grad_scale_dev, float grad_scale, void* stream);
+/* dsvc_adamw_step on `parts` slices of n floats that start `stride` floats apart in all four buffers (one tensor of every residual layer) */
+DSVC_API int dsvc_adamw_step_strided(float* params, const float* grads, float* exp_avg, float* exp_avg_sq, int64_t n, int64_t parts, int64_t stride, float lr,
+                                     float beta1, float beta2, float eps, float weight_decay, int64_t step, const float* grad_scale_dev, float grad_scale,
+                                     void* stream);
 /* clip_grad_norm_: *sqnorm_dev <- ||g||^2, *coef_dev <- min(1, max_norm / (||g|| + 1e-6)) */
 DSVC_API int dsvc_grad_clip_coef(const float* grads, int64_t n, float max_norm, float* sqnorm_dev, float* coef_dev, void* stream);
 
