@@ -10,7 +10,7 @@
 //   2. the sorted places are cut into chunks of equal length, whatever the tokens are; a wave adds one chunk's rows (a slice of 64 lanes' columns) in
 //      fp32 and writes the rows of dW whose places all lie in its chunk.  What a chunk boundary cuts goes to a partial row.  Waves of the same
 //      launch zero the rows of dW that have no place
-//   3. a run that spans chunks is closed by the chunk in which it starts: partial rows in chunk order, a fixed tree over four waves
+//   3. a run that spans chunks is closed by the chunk in which it starts: partial rows in chunk order, shared out to sixteen waves in fixed pieces
 // A token that fills the batch costs what a batch of different tokens costs.
 #include <math.h>
 
@@ -74,59 +74,55 @@ __global__ __launch_bounds__(256) void k_embed(const void* __restrict__ tokens, 
     }
 }
 
-// ---- 1. stable radix sort, 8 bits a pass ------------------------------------------------------------------------------------------------------
+// ---- 1. stable radix sort ---------------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ unsigned key_of(long long t, long long V, long long pad) { return t < 0 || t >= V || t == pad ? (unsigned)V : (unsigned)t; }
 
-// rank of every lane's digit among the equal digits of the wave's earlier items; cnt = this wave's 256 running counts
-__device__ __forceinline__ int wave_rank(int d, int lane, volatile int* cnt) {
+// rank of every lane's digit among the equal digits of the wave's earlier items; cnt = this wave's running counts
+template <class Count>
+__device__ __forceinline__ int wave_rank(int d, int bits, int lane, volatile Count* cnt) {
     unsigned long long same = ~0ull;
-#pragma unroll
-    for (int b = 0; b < 8; ++b) {
+    for (int b = 0; b < bits; ++b) {
         const unsigned long long set = __ballot((d >> b) & 1);
         same &= (d >> b) & 1 ? set : ~set;
     }
     const int before = cnt[d], below = __popcll(same & ((1ull << lane) - 1));
     __builtin_amdgcn_wave_barrier();
-    if (below == 0) cnt[d] = before + __popcll(same);
+    if (below == 0) cnt[d] = (Count)(before + __popcll(same));
     __builtin_amdgcn_wave_barrier();
     return before + below;
 }
 
-// NW waves' counts -> first slot of every (wave, digit): exclusive over digits, then over waves.  256 or more threads; tot: 256 ints
+// exclusive sum over the workgroup's threads (NW waves); tot: NW ints of LDS
 template <int NW>
-__device__ __forceinline__ void scan_counts(int (*cnt)[256], int* tot) {
-    const int t = threadIdx.x;
-    int run = 0;
-    if (t < 256) {
+__device__ __forceinline__ int block_scan(int v, int* tot) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int inc = v;
 #pragma unroll
-        for (int w = 0; w < NW; ++w) { const int c = cnt[w][t]; cnt[w][t] = run; run += c; }
-        tot[t] = run;
+    for (int k = 1; k < 64; k <<= 1) {
+        const int o = __shfl_up(inc, k);
+        if (lane >= k) inc += o;
     }
+    if (lane == 63) tot[wave] = inc;
     __syncthreads();
-    for (int k = 1; k < 256; k <<= 1) {
-        const int v = t < 256 && t >= k ? tot[t - k] : 0;
-        __syncthreads();
-        if (t < 256) tot[t] += v;
-        __syncthreads();
-    }
-    if (t < 256) {
-        const int first = tot[t] - run;
-#pragma unroll
-        for (int w = 0; w < NW; ++w) cnt[w][t] += first;
-    }
+    int before = 0;
+    for (int w = 0; w < NW; ++w) before += w < wave ? tot[w] : 0;
     __syncthreads();
+    return before + inc - v;
 }
 
-// up to 1024 IPT tokens in one workgroup: items stay in registers, each pass exchanges them through LDS
+// Up to 16384 tokens in one workgroup and one launch: items stay in registers, each pass exchanges them through LDS.  Digits of up to 10 bits: a table of
+// 256 rows and its ignored places (257 keys) is one pass.  Bound by one CU's latencies (8192 places of 257 keys: 17 us in two passes of 8 bits with the
+// digits scanned in 16 barriers, 11 us in one pass with shuffles).
+constexpr int ONE_MAX = 16384, ONE_BITS = 10;
 template <int IPT>
-__global__ __launch_bounds__(1024) void k_sort_one(const void* __restrict__ tokens, int i64, int n, long long V, long long pad, int passes, unsigned* __restrict__ keys,
+__global__ __launch_bounds__(1024) void k_sort_one(const void* __restrict__ tokens, int i64, int n, long long V, long long pad, int passes, int bits, unsigned* __restrict__ keys,
                                                    int* __restrict__ order) {
     extern __shared__ int sm[];
-    int(*cnt)[256] = (int(*)[256])sm;
-    int* tot = sm + 16 * 256;
-    unsigned* skey = (unsigned*)(tot + 256);
-    int* sidx = (int*)(skey + 1024 * IPT);
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, first = wave * 64 * IPT + lane;
+    unsigned* skey = (unsigned*)sm;
+    unsigned short* sidx = (unsigned short*)(skey + 1024 * IPT);
+    int* tot = (int*)(sidx + 1024 * IPT);
+    unsigned short* cnt = (unsigned short*)(tot + 16);           // [16][1 << bits]
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, first = wave * 64 * IPT + lane, bins = 1 << bits;
     unsigned key[IPT];
     int idx[IPT];
 #pragma unroll
@@ -135,18 +131,30 @@ __global__ __launch_bounds__(1024) void k_sort_one(const void* __restrict__ toke
         key[i] = idx[i] < n ? key_of(token_at(tokens, i64, idx[i]), V, pad) : (unsigned)V;       // (items behind the end stay behind all others: stable)
     }
     for (int p = 0; p < passes; ++p) {
-        for (int i = threadIdx.x; i < 16 * 256; i += 1024) sm[i] = 0;
+        const int shift = bits * p;
+        for (int i = threadIdx.x; i < 16 * bins / 2; i += 1024) ((int*)cnt)[i] = 0;
         __syncthreads();
         int rank[IPT];
 #pragma unroll
-        for (int i = 0; i < IPT; ++i) rank[i] = wave_rank((key[i] >> (8 * p)) & 255, lane, cnt[wave]);
+        for (int i = 0; i < IPT; ++i) rank[i] = wave_rank((key[i] >> shift) & (bins - 1), bits, lane, (volatile unsigned short*)(cnt + wave * bins));
         __syncthreads();
-        scan_counts<16>(cnt, tot);
+        // counts -> first slot of every (wave, digit): over the waves, then over the digits.  (At most 16384 items: slots fit 16 bits.)
+        int run = 0, c[16];
+        if ((int)threadIdx.x < bins) {
+#pragma unroll
+            for (int w = 0; w < 16; ++w) { c[w] = cnt[w * bins + threadIdx.x]; run += c[w]; }
+        }
+        int at = block_scan<16>(run, tot);
+        if ((int)threadIdx.x < bins) {
+#pragma unroll
+            for (int w = 0; w < 16; ++w) { cnt[w * bins + threadIdx.x] = (unsigned short)at; at += c[w]; }
+        }
+        __syncthreads();
 #pragma unroll
         for (int i = 0; i < IPT; ++i) {
-            const int at = cnt[wave][(key[i] >> (8 * p)) & 255] + rank[i];
-            skey[at] = key[i];
-            sidx[at] = idx[i];
+            const int to = cnt[wave * bins + ((key[i] >> shift) & (bins - 1))] + rank[i];
+            skey[to] = key[i];
+            sidx[to] = (unsigned short)idx[i];
         }
         __syncthreads();
 #pragma unroll
@@ -154,7 +162,6 @@ __global__ __launch_bounds__(1024) void k_sort_one(const void* __restrict__ toke
             key[i] = skey[first + i * 64];
             idx[i] = sidx[first + i * 64];
         }
-        __syncthreads();
     }
 #pragma unroll
     for (int i = 0; i < IPT; ++i)
@@ -164,75 +171,92 @@ __global__ __launch_bounds__(1024) void k_sort_one(const void* __restrict__ toke
         }
 }
 
-// more tokens: blocks of 4096.  hist[digit][block]; src_keys == nullptr: the first pass, from the tokens themselves
-constexpr int SORT_BLOCK = 4096;
+// More tokens: blocks of 256 IPT, up to 8 bits a pass, counts as hist[digit][block].  The first pass reads the tokens themselves (keys == nullptr).
+// Up to 64 blocks a block finds its first slots from the whole table of counts itself (64 KiB in L2): two launches a pass.  Beyond, the table is
+// scanned by a launch of its own.  (Counting a pass's digits while the pass before it scatters saves a launch, but its atomics meet at a skewed
+// text's few digits: 32768 places 31 us instead of 7.5 + 4.7.)
+constexpr int FEW_BLOCKS = 64;
 struct SortSrc { const void* tokens; int i64; long long V, pad; const unsigned* keys; const int* order; };
 __device__ __forceinline__ void sort_load(const SortSrc& s, long long i, long long n, unsigned& key, int& idx) {
     if (i >= n) { key = ~0u; idx = 0; return; }
     key = s.keys ? s.keys[i] : key_of(token_at(s.tokens, s.i64, i), s.V, s.pad);
     idx = s.keys ? s.order[i] : (int)i;
 }
-__global__ __launch_bounds__(256) void k_sort_hist(SortSrc s, long long n, int shift, int* __restrict__ hist) {
+template <int IPT>
+__global__ __launch_bounds__(256) void k_sort_hist(SortSrc s, long long n, int shift, int mask, int* __restrict__ hist, int ld) {
     __shared__ int cnt[256];
     cnt[threadIdx.x] = 0;
     __syncthreads();
-#pragma unroll 4
-    for (int i = 0; i < SORT_BLOCK / 256; ++i) {
-        const long long at = (long long)blockIdx.x * SORT_BLOCK + i * 256 + threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < IPT; ++i) {
+        const long long at = (long long)blockIdx.x * (256 * IPT) + i * 256 + threadIdx.x;
         unsigned key; int idx;
         sort_load(s, at, n, key, idx);
-        if (at < n) atomicAdd(&cnt[(key >> shift) & 255], 1);
+        if (at < n) atomicAdd(&cnt[(key >> shift) & mask], 1);
     }
     __syncthreads();
-    hist[(long long)threadIdx.x * gridDim.x + blockIdx.x] = cnt[threadIdx.x];
+    hist[(long long)threadIdx.x * ld + blockIdx.x] = cnt[threadIdx.x];
 }
 __global__ __launch_bounds__(1024) void k_sort_scan(int* __restrict__ hist, int n) {      // exclusive scan in place
-    __shared__ int wsum[16];
+    __shared__ int tot[16];
     __shared__ int carry;
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    if (t == 0) carry = 0;
+    if (threadIdx.x == 0) carry = 0;
     __syncthreads();
     for (int base = 0; base < n; base += 8192) {
         int v[8], sum = 0;
-        const int at = base + t * 8;
+        const int at = base + threadIdx.x * 8;
 #pragma unroll
         for (int i = 0; i < 8; ++i) { v[i] = at + i < n ? hist[at + i] : 0; sum += v[i]; }
-        int inc = sum;
-        for (int k = 1; k < 64; k <<= 1) { const int o = __shfl_up(inc, k); if (lane >= k) inc += o; }
-        if (lane == 63) wsum[wave] = inc;
+        int run = block_scan<16>(sum, tot) + carry;
         __syncthreads();
-        int run = carry + inc - sum;
-        for (int w = 0; w < wave; ++w) run += wsum[w];
-        __syncthreads();
-        if (t == 1023) carry = run + sum;
+        if (threadIdx.x == 1023) carry = run + sum;
 #pragma unroll
         for (int i = 0; i < 8; ++i) { if (at + i < n) hist[at + i] = run; run += v[i]; }
         __syncthreads();
     }
 }
-__global__ __launch_bounds__(256) void k_sort_scatter(SortSrc s, long long n, int shift, const int* __restrict__ hist, unsigned* __restrict__ keys, int* __restrict__ order) {
+// FEW: hist holds counts (ld = FEW_BLOCKS); else first slots
+template <int IPT, bool FEW>
+__global__ __launch_bounds__(256) void k_sort_scatter(SortSrc s, long long n, int shift, int bits, const int* __restrict__ hist, int ld, unsigned* __restrict__ keys,
+                                                      int* __restrict__ order) {
     __shared__ int cnt[4][256];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    __shared__ int tot[4];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, mask = (1 << bits) - 1;
     for (int w = 0; w < 4; ++w) cnt[w][threadIdx.x] = 0;
     __syncthreads();
-    constexpr int IPT = SORT_BLOCK / 256;
-    const long long first = (long long)blockIdx.x * SORT_BLOCK + wave * 64 * IPT + lane;
+    const long long first = (long long)blockIdx.x * (256 * IPT) + wave * 64 * IPT + lane;
     unsigned key[IPT];
     int idx[IPT], rank[IPT];
 #pragma unroll
     for (int i = 0; i < IPT; ++i) sort_load(s, first + i * 64, n, key[i], idx[i]);
+    int run = 0;
+    if (FEW) {
+        int all = 0;
+        const int4* h = (const int4*)(hist + threadIdx.x * FEW_BLOCKS);
 #pragma unroll
-    for (int i = 0; i < IPT; ++i) rank[i] = wave_rank((key[i] >> shift) & 255, lane, cnt[wave]);
+        for (int q = 0; q < FEW_BLOCKS / 4; ++q) {
+            const int4 v = h[q];
+            const int e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int c = 4 * q + k < (int)gridDim.x ? e[k] : 0;
+                all += c;
+                run += 4 * q + k < (int)blockIdx.x ? c : 0;
+            }
+        }
+        run += block_scan<4>(all, tot);
+    } else run = hist[(long long)threadIdx.x * ld + blockIdx.x];
+#pragma unroll
+    for (int i = 0; i < IPT; ++i) rank[i] = wave_rank((key[i] >> shift) & mask, bits, lane, (volatile int*)cnt[wave]);
     __syncthreads();
-    // this block's slots of a digit start at hist[digit][block]; the waves' shares follow one another.  Items behind the end have the highest
-    // digit and come last in the last block: they take no slot of another's
-    int run = hist[(long long)threadIdx.x * gridDim.x + blockIdx.x];
+    // this block's slots of a digit start at `run`; the waves' shares follow one another.  Items behind the end have the highest digit and come
+    // last in the last block: they take no slot of another's
     for (int w = 0; w < 4; ++w) { const int c = cnt[w][threadIdx.x]; cnt[w][threadIdx.x] = run; run += c; }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < IPT; ++i)
         if (first + i * 64 < n) {
-            const int at = cnt[wave][(key[i] >> shift) & 255] + rank[i];
+            const int at = cnt[wave][(key[i] >> shift) & mask] + rank[i];
             keys[at] = key[i];
             order[at] = idx[i];
         }
@@ -245,7 +269,7 @@ struct SegArgs {
     const unsigned* keys; const int* order;
     long long n;
     unsigned V;
-    int H, chunk, slices;                    // chunk <= 64 places; a slice = 64 lanes' columns
+    int H, chunk, slices;                    // places of a chunk; a slice = 64 lanes' columns
     long long n_chunks;
     const void* dy; long long dy_ld;
     void* dw; long long dw_ld;
@@ -335,81 +359,97 @@ __global__ __launch_bounds__(256) void k_seg_sum(const SegArgs a) {
     }
     const long long c = unit / a.slices, r0 = c * a.chunk;
     const int slice = (int)(unit - c * a.slices), c0 = slice * 64 * VEC + (VECTOR ? lane * VEC : lane);
-    const int rows = (int)(a.n - r0 < a.chunk ? a.n - r0 : a.chunk);
-    const unsigned kk = lane < rows ? a.keys[r0 + lane] : a.V;
-    const int oo = lane < rows ? a.order[r0 + lane] : 0;
+    const long long r1 = a.n - r0 < a.chunk ? a.n : r0 + a.chunk;
     const unsigned none = ~0u;
-    const unsigned prev = r0 > 0 ? a.keys[r0 - 1] : none, next = r0 + rows < a.n ? a.keys[r0 + rows] : none;
+    const unsigned prev = r0 > 0 ? a.keys[r0 - 1] : none, next = r1 < a.n ? a.keys[r1] : none;
     const D* dy = (const D*)a.dy;
     float acc[VEC];
 #pragma unroll
     for (int e = 0; e < VEC; ++e) acc[e] = 0.f;
-    unsigned cur = (unsigned)__builtin_amdgcn_readfirstlane((int)kk);
-    if (cur == a.V) return;                  // everything from here on is ignored
-    bool from_prev = prev == cur;
+    unsigned cur = none;                     // the run that is being added up, and whether it came from the chunk before
+    bool from_prev = false;
     constexpr int R = 8;                     // rows in flight
-    for (int i0 = 0; i0 < rows; i0 += R) {
-        float v[R][VEC];
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            const int i = i0 + r < rows ? i0 + r : rows - 1;
-            load_row<D, VEC, VECTOR>(dy + (long long)__builtin_amdgcn_readlane(oo, i) * a.dy_ld, c0, a.H, v[r]);
+    for (long long base = r0; base < r1; base += 64) {
+        const int rows = r1 - base < 64 ? (int)(r1 - base) : 64;
+        const unsigned kk = lane < rows ? a.keys[base + lane] : a.V;
+        const int oo = lane < rows ? a.order[base + lane] : 0;
+        if (base == r0) {
+            cur = (unsigned)__builtin_amdgcn_readfirstlane((int)kk);
+            if (cur == a.V) return;          // everything from here on is ignored
+            from_prev = prev == cur;
         }
+        for (int i0 = 0; i0 < rows; i0 += R) {
+            float v[R][VEC];
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            if (i0 + r >= rows) break;
-            const unsigned k = (unsigned)__builtin_amdgcn_readlane((int)kk, i0 + r);
-            if (k != cur) {                  // the run of `cur` ends here
-                if (from_prev) {
-                    if (c0 < a.H) store_row<float, VEC, VECTOR>(a.part + (c * 2) * a.H, c0, a.H, acc);
-                } else write_dw<O, VEC, VECTOR>(a, cur, c0, acc);
-                from_prev = false;
-                cur = k;
-                if (cur == a.V) return;
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) acc[e] = 0.f;
+            for (int r = 0; r < R; ++r) {
+                const int i = i0 + r < rows ? i0 + r : rows - 1;
+                load_row<D, VEC, VECTOR>(dy + (long long)__builtin_amdgcn_readlane(oo, i) * a.dy_ld, c0, a.H, v[r]);
             }
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) acc[e] += v[r][e];
+            for (int r = 0; r < R; ++r) {
+                if (i0 + r >= rows) break;
+                const unsigned k = (unsigned)__builtin_amdgcn_readlane((int)kk, i0 + r);
+                if (k != cur) {              // the run of `cur` ends here
+                    if (from_prev) store_row<float, VEC, VECTOR>(a.part + (c * 2) * a.H, c0, a.H, acc);
+                    else write_dw<O, VEC, VECTOR>(a, cur, c0, acc);
+                    from_prev = false;
+                    cur = k;
+                    if (cur == a.V) return;
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) acc[e] = 0.f;
+                }
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) acc[e] += v[r][e];
+            }
         }
     }
     if (from_prev || next == cur) store_row<float, VEC, VECTOR>(a.part + (c * 2 + (from_prev ? 0 : 1)) * a.H, c0, a.H, acc);
     else write_dw<O, VEC, VECTOR>(a, cur, c0, acc);
 }
 
-// ---- 3. runs that span chunks: grid (chunks, slices), four waves -----------------------------------------------------------------------------
+// ---- 3. runs that span chunks: grid (chunks, slices), sixteen waves.  Most blocks find nothing to close, most runs a few chunks: latency counts, so the
+// lanes of a wave look at the first places of 64 chunks at once and only longer runs are searched ----
+constexpr int JOIN_WAVES = 8;
 template <int TO, int VEC, bool VECTOR>
-__global__ __launch_bounds__(256) void k_seg_join(const SegArgs a) {
+__global__ __launch_bounds__(JOIN_WAVES * 64) void k_seg_join(const SegArgs a) {
     typedef typename Elem<TO>::type O;
     const long long c = blockIdx.x, r0 = c * a.chunk, r1 = r0 + a.chunk;
-    if (r1 >= a.n) return;                   // the last chunk hands nothing on
-    const unsigned key = a.keys[r1 - 1];
-    if (key == a.V || a.keys[r1] != key || (r0 > 0 && a.keys[r0 - 1] == key)) return;      // no run starts here and goes on
-    long long lo = r1, hi = a.n;             // first place behind the run
-    while (lo < hi) {
-        const long long mid = (lo + hi) >> 1;
-        if (a.keys[mid] <= key) lo = mid + 1; else hi = mid;
-    }
-    const long long last = (lo - 1) / a.chunk, terms = last - c + 1;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c0 = blockIdx.y * 64 * VEC + (VECTOR ? lane * VEC : lane);
-    const long long per = (terms + 3) / 4, t0 = wave * per, t1 = t0 + per < terms ? t0 + per : terms;
+    if (r1 >= a.n) return;                   // the last chunk hands nothing on
+    const long long probe = r1 + (long long)lane * a.chunk;
+    const unsigned key = a.keys[r1 - 1], before = r0 > 0 ? a.keys[r0 - 1] : ~0u, there = probe < a.n ? a.keys[probe] : ~0u;
+    const unsigned long long on = __ballot(there == key);
+    if (key == a.V || !(on & 1) || before == key) return;        // no run starts here and goes on
+    long long terms;                         // chunks that the run touches
+    if (~on) terms = 1 + __ffsll((long long)~on) - 1;
+    else {
+        long long lo = r1 + 63 * (long long)a.chunk, hi = a.n;   // first place behind the run
+        while (lo < hi) {
+            const long long mid = (lo + hi) >> 1;
+            if (a.keys[mid] <= key) lo = mid + 1; else hi = mid;
+        }
+        terms = (lo - 1) / a.chunk - c + 1;
+    }
+    const long long per = (terms + JOIN_WAVES - 1) / JOIN_WAVES, t0 = wave * per, t1 = t0 + per < terms ? t0 + per : terms;
     float acc[VEC];
 #pragma unroll
     for (int e = 0; e < VEC; ++e) acc[e] = 0.f;
-#pragma unroll 4
+#pragma unroll (64 / VEC)
     for (long long t = t0; t < t1; ++t) {
         float v[VEC];
         load_row<float, VEC, VECTOR>(a.part + ((c + t) * 2 + (t == 0 ? 1 : 0)) * a.H, c0, a.H, v);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) acc[e] += v[e];
     }
-    __shared__ float red[4][VEC][64];
+    __shared__ float red[JOIN_WAVES][VEC][64];
 #pragma unroll
     for (int e = 0; e < VEC; ++e) red[wave][e][lane] = acc[e];
     __syncthreads();
     if (wave) return;
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) acc[e] = (red[0][e][lane] + red[1][e][lane]) + (red[2][e][lane] + red[3][e][lane]);
+    for (int w = 1; w < JOIN_WAVES; ++w)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) acc[e] += red[w][e][lane];
     write_dw<O, VEC, VECTOR>(a, key, c0, acc);
 }
 
@@ -418,37 +458,63 @@ inline int size_of(int dtype) { return dtype == F32 ? 4 : 2; }
 inline bool known(int dtype) { return dtype == F32 || dtype == F16 || dtype == BF16; }
 
 struct GradPlan {
-    int passes, one, ipt, chunk;
+    int passes, bits, one, ipt, chunk;
     long long n_chunks, blocks, off_k[2], off_o[2], off_hist, off_part, bytes;
 };
 
-int grad_plan(int64_t n, int64_t V, int32_t H, GradPlan* p) {
+int grad_plan(int64_t n, int64_t V, int32_t H, int esize, GradPlan* p) {
     if (n < 0 || n > (1LL << 28)) return fail(DSVC_EINVAL, "embed_tokens_grad: %lld tokens", (long long)n);
     if (V < 1 || V > (1LL << 30)) return fail(DSVC_EINVAL, "embed_tokens_grad: %lld rows", (long long)V);
     if (H < 1 || H > (1 << 20)) return fail(DSVC_EINVAL, "embed_tokens_grad: %d columns", H);
     *p = GradPlan{};
     int bits = 1;
     while ((V >> bits) != 0) ++bits;         // keys 0 ... V
-    p->passes = (bits + 7) / 8;
-    p->one = n <= 16384;
-    p->ipt = n <= 1024 ? 1 : n <= 2048 ? 2 : n <= 4096 ? 4 : n <= 8192 ? 8 : 16;
-    p->chunk = 32;
+    // one workgroup: 8192 places in one pass 11 us, 16384 in two 47 us, where two passes of two launches take 25 us
+    p->one = bits <= ONE_BITS ? n <= ONE_MAX : n <= ONE_MAX / 4;
+    const int most = p->one ? ONE_BITS : 8;
+    p->passes = (bits + most - 1) / most;
+    p->bits = (bits + p->passes - 1) / p->passes;
+    p->ipt = p->one ? (n <= 1024 ? 1 : n <= 2048 ? 2 : n <= 4096 ? 4 : n <= 8192 ? 8 : 16) : (n <= FEW_BLOCKS * 1024 ? 4 : n <= FEW_BLOCKS * 2048 ? 8 : 16);
+    // chunks: enough waves to fill the chip (16 a CU) from few tokens, few partial rows in a run from many
+    const long long slices = (H + 64 * (16 / esize) - 1) / (64 * (16 / esize));
+    const long long want = n * slices / 4096;
+    p->chunk = (int)(want < 8 ? 8 : want > 2048 ? 2048 : (want + 7) / 8 * 8);
     p->n_chunks = (n + p->chunk - 1) / p->chunk;
-    p->blocks = (n + SORT_BLOCK - 1) / SORT_BLOCK;
+    p->blocks = (n + 256 * p->ipt - 1) / (256 * p->ipt);
     long long at = 0;
     auto take = [&](long long bytes) { const long long o = at; at += (bytes + 255) / 256 * 256; return o; };
     for (int i = 0; i < (p->one ? 1 : 2); ++i) { p->off_k[i] = take(n * 4); p->off_o[i] = take(n * 4); }
-    if (!p->one) p->off_hist = take(256 * p->blocks * 4);
+    if (!p->one) p->off_hist = take(256 * (p->blocks <= FEW_BLOCKS ? FEW_BLOCKS : p->blocks) * 4);
     p->off_part = take(p->n_chunks * 2 * H * 4);
     p->bytes = at < 256 ? 256 : at;
     return DSVC_OK;
 }
 
 template <int IPT>
-int sort_one(const void* tokens, int i64, int n, long long V, long long pad, int passes, unsigned* keys, int* order, hipStream_t st) {
-    constexpr int LDS = (16 * 256 + 256 + 2 * 1024 * IPT) * 4;
-    if (LDS > 64 * 1024) DSVC_HIP(hipFuncSetAttribute((const void*)k_sort_one<IPT>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS));
-    hipLaunchKernelGGL(k_sort_one<IPT>, dim3(1), dim3(1024), LDS, st, tokens, i64, n, V, pad, passes, keys, order);
+int sort_one(const void* tokens, int i64, int n, long long V, long long pad, const GradPlan& p, unsigned* keys, int* order, hipStream_t st) {
+    const int lds = 1024 * IPT * 6 + 64 + 32 * (1 << p.bits);
+    if (lds > 64 * 1024) DSVC_HIP(hipFuncSetAttribute((const void*)k_sort_one<IPT>, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+    hipLaunchKernelGGL(k_sort_one<IPT>, dim3(1), dim3(1024), lds, st, tokens, i64, n, V, pad, p.passes, p.bits, keys, order);
+    DSVC_HIP(hipGetLastError());
+    return DSVC_OK;
+}
+// returns through `at` which of the two buffers holds the result
+template <int IPT>
+int sort_many(const void* tokens, int i64, long long n, long long V, long long pad, const GradPlan& p, int* hist, unsigned* const (&keys)[2], int* const (&order)[2], int* at,
+              hipStream_t st) {
+    const dim3 grid((unsigned)p.blocks), block(256);
+    const bool few = p.blocks <= FEW_BLOCKS;
+    const int mask = (1 << p.bits) - 1, ld = few ? FEW_BLOCKS : (int)p.blocks;
+    for (int k = 0; k < p.passes; ++k) {
+        const SortSrc s{tokens, i64, V, pad, k ? keys[(k + 1) & 1] : nullptr, k ? order[(k + 1) & 1] : nullptr};
+        *at = k & 1;
+        hipLaunchKernelGGL(k_sort_hist<IPT>, grid, block, 0, st, s, n, p.bits * k, mask, hist, ld);
+        if (few) hipLaunchKernelGGL((k_sort_scatter<IPT, true>), grid, block, 0, st, s, n, p.bits * k, p.bits, hist, ld, keys[*at], order[*at]);
+        else {
+            hipLaunchKernelGGL(k_sort_scan, dim3(1), dim3(1024), 0, st, hist, (int)(256 * p.blocks));
+            hipLaunchKernelGGL((k_sort_scatter<IPT, false>), grid, block, 0, st, s, n, p.bits * k, p.bits, hist, ld, keys[*at], order[*at]);
+        }
+    }
     DSVC_HIP(hipGetLastError());
     return DSVC_OK;
 }
@@ -459,7 +525,7 @@ int segments(SegArgs a, hipStream_t st) {
     const long long zero = a.accumulate ? 0 : ((long long)a.V + ZERO_ROWS - 1) / ZERO_ROWS, units = a.n_chunks * a.slices + zero;
     if (units >= (1LL << 26)) return fail(DSVC_EINVAL, "embed_tokens_grad: %lld work items", units);
     if (units) hipLaunchKernelGGL((k_seg_sum<TD, TO, VEC, VECTOR>), dim3((unsigned)((units + 3) / 4)), dim3(256), 0, st, a);
-    if (a.n_chunks > 1) hipLaunchKernelGGL((k_seg_join<TO, VEC, VECTOR>), dim3((unsigned)(a.n_chunks - 1), a.slices), dim3(256), 0, st, a);
+    if (a.n_chunks > 1) hipLaunchKernelGGL((k_seg_join<TO, VEC, VECTOR>), dim3((unsigned)(a.n_chunks - 1), a.slices), dim3(JOIN_WAVES * 64), 0, st, a);
     DSVC_HIP(hipGetLastError());
     return DSVC_OK;
 }
@@ -502,7 +568,7 @@ int dsvc_embed_tokens(const void* tokens, int32_t tokens_i64, int64_t n, const v
 int dsvc_embed_tokens_grad_workspace(int64_t n, int64_t vocab, int32_t H, int64_t* bytes) {
     if (!bytes) return fail(DSVC_EINVAL, "null argument");
     GradPlan p;
-    DSVC_TRY(grad_plan(n, vocab, H, &p));
+    DSVC_TRY(grad_plan(n, vocab, H, 2, &p));                    // (16-bit gradients have the shortest chunks, and so the most partial rows)
     *bytes = p.bytes;
     return DSVC_OK;
 }
@@ -510,7 +576,7 @@ int dsvc_embed_tokens_grad_workspace(int64_t n, int64_t vocab, int32_t H, int64_
 int dsvc_embed_tokens_grad(const void* tokens, int32_t tokens_i64, int64_t n, const void* dy, int64_t dy_ld, int32_t dy_dtype, int64_t vocab, int32_t H, float scale,
                            int64_t padding_idx, void* dw, int64_t dw_ld, int32_t dw_dtype, int32_t accumulate, void* workspace, int64_t workspace_bytes, void* stream) {
     GradPlan p;
-    DSVC_TRY(grad_plan(n, vocab, H, &p));
+    DSVC_TRY(grad_plan(n, vocab, H, dy_dtype == F32 ? 4 : 2, &p));
     if (!known(dy_dtype) || (dw_dtype != dy_dtype && dw_dtype != F32)) return fail(DSVC_EINVAL, "embed_tokens_grad: types %d -> %d", dy_dtype, dw_dtype);
     if ((dy_ld < H && n > 1) || (dw_ld < H && vocab > 1)) return fail(DSVC_EINVAL, "embed_tokens_grad: row strides %lld, %lld of %d columns", (long long)dy_ld, (long long)dw_ld, H);
     if (!isfinite(scale)) return fail(DSVC_EINVAL, "embed_tokens_grad: scale %g", scale);
@@ -524,21 +590,16 @@ int dsvc_embed_tokens_grad(const void* tokens, int32_t tokens_i64, int64_t n, co
     int at = 0;
     if (n > 0 && p.one) {
         const int m = (int)n;
-        if (p.ipt == 1) DSVC_TRY(sort_one<1>(tokens, i64, m, vocab, padding_idx, p.passes, keys[0], order[0], st));
-        else if (p.ipt == 2) DSVC_TRY(sort_one<2>(tokens, i64, m, vocab, padding_idx, p.passes, keys[0], order[0], st));
-        else if (p.ipt == 4) DSVC_TRY(sort_one<4>(tokens, i64, m, vocab, padding_idx, p.passes, keys[0], order[0], st));
-        else if (p.ipt == 8) DSVC_TRY(sort_one<8>(tokens, i64, m, vocab, padding_idx, p.passes, keys[0], order[0], st));
-        else DSVC_TRY(sort_one<16>(tokens, i64, m, vocab, padding_idx, p.passes, keys[0], order[0], st));
+        if (p.ipt == 1) DSVC_TRY(sort_one<1>(tokens, i64, m, vocab, padding_idx, p, keys[0], order[0], st));
+        else if (p.ipt == 2) DSVC_TRY(sort_one<2>(tokens, i64, m, vocab, padding_idx, p, keys[0], order[0], st));
+        else if (p.ipt == 4) DSVC_TRY(sort_one<4>(tokens, i64, m, vocab, padding_idx, p, keys[0], order[0], st));
+        else if (p.ipt == 8) DSVC_TRY(sort_one<8>(tokens, i64, m, vocab, padding_idx, p, keys[0], order[0], st));
+        else DSVC_TRY(sort_one<16>(tokens, i64, m, vocab, padding_idx, p, keys[0], order[0], st));
     } else if (n > 0) {
         int* hist = (int*)(ws + p.off_hist);
-        for (int k = 0; k < p.passes; ++k) {
-            const SortSrc s{tokens, i64, vocab, padding_idx, k ? keys[(k + 1) & 1] : nullptr, k ? order[(k + 1) & 1] : nullptr};
-            at = k & 1;
-            hipLaunchKernelGGL(k_sort_hist, dim3((unsigned)p.blocks), dim3(256), 0, st, s, n, 8 * k, hist);
-            hipLaunchKernelGGL(k_sort_scan, dim3(1), dim3(1024), 0, st, hist, (int)(256 * p.blocks));
-            hipLaunchKernelGGL(k_sort_scatter, dim3((unsigned)p.blocks), dim3(256), 0, st, s, n, 8 * k, hist, keys[at], order[at]);
-        }
-        DSVC_HIP(hipGetLastError());
+        if (p.ipt == 4) DSVC_TRY(sort_many<4>(tokens, i64, n, vocab, padding_idx, p, hist, keys, order, &at, st));
+        else if (p.ipt == 8) DSVC_TRY(sort_many<8>(tokens, i64, n, vocab, padding_idx, p, hist, keys, order, &at, st));
+        else DSVC_TRY(sort_many<16>(tokens, i64, n, vocab, padding_idx, p, hist, keys, order, &at, st));
     }
     const SegArgs a{keys[at], order[at], n, (unsigned)vocab, H, p.chunk, 0, p.n_chunks, dy, dy_ld, dw, dw_ld, (float*)(ws + p.off_part), scale, accumulate != 0};
     const int ds = size_of(dy_dtype), os = size_of(dw_dtype);

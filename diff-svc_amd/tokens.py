@@ -59,16 +59,18 @@ def _padding(padding_idx, vocab):
 def _lookup(tokens, weight, scale, flag):
     if weight.dim() != 2 or not weight.shape[0] or not weight.shape[1]:
         raise ValueError("the table must be [rows, columns], got %s" % (tuple(weight.shape),))
-    if weight.dtype not in DTYPES:
+    dtype = DTYPES.get(weight.dtype)
+    if dtype is None:
         raise TypeError("diffsvc_amd: tables are float32, float16 or bfloat16, got %s" % weight.dtype)
     _check_tokens(tokens, weight)
     V, H = weight.shape
     w, t = rows_of(weight), tokens if tokens.is_contiguous() else tokens.contiguous()
-    out = torch.empty(tokens.shape + (H,), device=w.device, dtype=w.dtype)
+    out = w.new_empty((*tokens.shape, H))
     here, stream = on_device(w)
     with here:
-        check(lib().dsvc_embed_tokens(t.data_ptr(), t.dtype == torch.int64, t.numel(), w.data_ptr(), w.stride(0), V, H, DTYPES[w.dtype], scale,
-                                      out.data_ptr(), H, None if flag is None else flag.data_ptr(), stream))
+        rc = lib().dsvc_embed_tokens(t.data_ptr(), t.dtype is torch.int64, t.numel(), w.data_ptr(), w.stride(0), V, H, dtype, scale, out.data_ptr(), H,
+                                     None if flag is None else flag.data_ptr(), stream)
+    check(rc)
     return out
 
 
@@ -94,13 +96,15 @@ def embed_tokens_grad(tokens, dy, vocab, scale=1.0, padding_idx=None, out=None, 
         raise ValueError("out must be [%d, %d] of %s or float32 on %s" % (vocab, H, d.dtype, d.device))
     elif (H > 1 and out.stride(1) != 1) or (vocab > 1 and out.stride(0) < H):
         raise ValueError("out needs rows of unit stride that do not overlap, got strides %s" % (out.stride(),))
+    L = lib()
+    need = ctypes.c_int64(0)
+    check(L.dsvc_embed_tokens_grad_workspace(n, vocab, H, ctypes.byref(need)))
+    ws = torch.empty(need.value, device=d.device, dtype=torch.uint8)
     here, stream = on_device(d)
     with here:
-        need = ctypes.c_int64(0)
-        check(lib().dsvc_embed_tokens_grad_workspace(n, vocab, H, ctypes.byref(need)))
-        ws = torch.empty(need.value, device=d.device, dtype=torch.uint8)
-        check(lib().dsvc_embed_tokens_grad(t.data_ptr(), t.dtype == torch.int64, n, d.data_ptr(), d.stride(0), DTYPES[d.dtype], vocab, H, scale, pad,
-                                           out.data_ptr(), out.stride(0), DTYPES[out.dtype], accumulate, ws.data_ptr(), need.value, stream))
+        rc = L.dsvc_embed_tokens_grad(t.data_ptr(), t.dtype is torch.int64, n, d.data_ptr(), d.stride(0), DTYPES[d.dtype], vocab, H, scale, pad,
+                                      out.data_ptr(), out.stride(0), DTYPES[out.dtype], accumulate, ws.data_ptr(), need.value, stream)
+    check(rc)
     return out
 
 
