@@ -36,6 +36,10 @@ typedef const half8 __attribute__((address_space(3))) * lds_half8;
 
 constexpr float X_SCALE = 4096.f, A_SCALE = 1024.f;
 constexpr int PAD = 128;                     // rows and columns of every intermediate are padded to this
+// Padded elements up to which one workgroup takes a matrix of up to 64 rows.  fp32, one workgroup against 17 launches (GPU time; the host takes 70 us to
+// launch them): [1, 1] 24 / 71 us, [64, 64] x 8 27 / 76, [64, 256] 52 / 80, [32, 500] 72 / 88, [64, 1024] 163 / 103; [48, 64] x 2000 197 / 1162
+constexpr long long ONE_WORK = 16384;
+constexpr int ONE_LDS = 156 * 1024;          // its LDS (the rest: static)
 constexpr int SUM_BLOCKS = 256;              // partial sums of squares per matrix
 
 enum { F32 = DSVC_DTYPE_F32, F16 = DSVC_DTYPE_F16, BF16 = DSVC_DTYPE_BF16 };
@@ -178,6 +182,32 @@ __global__ __launch_bounds__(256) void k_ns_prep(const void* __restrict__ in, Vi
 // ---- the products ----------------------------------------------------------------------------------------------------------------------
 enum { GRAM, POLY, FULL, FINAL };
 
+// the caller's tensor: the result, or (mu.mom) the parameter, out <- (1 - lr wd) out - lr result
+struct Output {
+    void* out; View ov;
+    int dtype, m, n, tall;
+    MuonArgs mu;
+};
+// 32 x 32 block (bi, bj) of matrix b, scaled by c: register r of a lane = row 8 (r >> 2) + 4 (lane >> 5) + (r & 3), column lane & 31
+__device__ __forceinline__ void store_result(const Output& o, int b, int bi, int bj, int lane, const f32x16& acc, float c) {
+    const int col = 32 * bj + (lane & 31);
+    if (col >= o.n) return;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        const int row = 32 * bi + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
+        if (row >= o.m) continue;
+        const long long at = b * o.ov.bs + (o.tall ? col * o.ov.ld + row : row * o.ov.ld + col);
+        float v = acc[r] * c;
+        if (o.mu.mom) {
+            const float p = o.dtype == F32 ? ((float*)o.out)[at] : o.dtype == F16 ? (float)((_Float16*)o.out)[at] : (float)((__bf16*)o.out)[at];
+            v = fmaf(-o.mu.lr, v, (1.f - o.mu.lr * o.mu.wd) * p);
+        }
+        if (o.dtype == F32) ((float*)o.out)[at] = v;
+        else if (o.dtype == F16) ((_Float16*)o.out)[at] = (_Float16)v;
+        else ((__bf16*)o.out)[at] = (__bf16)v;
+    }
+}
+
 struct NsGemm {
     const _Float16 *a, *b;                   // fragment-order operands, rows x K each: result[i][j] = sum_k a[i][k] b[j][k]
     long long a_bs, b_bs;                    // halfs per matrix
@@ -192,10 +222,7 @@ struct NsGemm {
     float c0, c1, c2;                        // POLY: c0 on the diagonal, c1 A, c2 acc; others: c2 acc
     const Scalars* sc;
     int step, dec;                           // e_k = max(0, e0 - k dec)
-    // FINAL
-    void* out; View ov;
-    int dtype, m, n, tall;
-    MuonArgs mu;                             // mu.mom: out is the parameter, out <- (1 - lr wd) out - lr result
+    Output fin;                              // FINAL
 };
 
 template <int N> __device__ __forceinline__ void wait_vm_lgkm() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory"); }
@@ -427,7 +454,7 @@ __global__ __launch_bounds__(C::NW * 64) void k_ns_gemm(const NsGemm g) {
     }
     if (grp > 0) return;
 
-    // ---- epilogue: register r of a lane = row 8 (r >> 2) + 4 (lane >> 5) + (r & 3), column lane & 31 ----
+    // ---- epilogue: registers and lanes as in store_result ----
     const int e0 = g.sc[b].e0, ek = max(0, e0 - g.step * g.dec), ek1 = max(0, e0 - (g.step + 1) * g.dec);
     float c2 = g.c2;
     if (MODE == GRAM) c2 = ldexpf(c2, -2 * ek);
@@ -444,22 +471,7 @@ __global__ __launch_bounds__(C::NW * 64) void k_ns_gemm(const NsGemm g) {
         for (int j = 0; j < TN; ++j) {
             const int bi = ti * RA + wr * TM + i, bj = tj * RB + wc * TN + j;      // 32-blocks of the result
             if constexpr (MODE == FINAL) {
-                const int col = 32 * bj + (lane & 31);
-                if (col >= g.n) continue;
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int row = 32 * bi + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
-                    if (row >= g.m) continue;
-                    const long long at = b * g.ov.bs + (g.tall ? col * g.ov.ld + row : row * g.ov.ld + col);
-                    float v = acc[i][j][r] * c2;
-                    if (g.mu.mom) {
-                        const float p = g.dtype == F32 ? ((float*)g.out)[at] : g.dtype == F16 ? (float)((_Float16*)g.out)[at] : (float)((__bf16*)g.out)[at];
-                        v = fmaf(-g.mu.lr, v, (1.f - g.mu.lr * g.mu.wd) * p);
-                    }
-                    if (g.dtype == F32) ((float*)g.out)[at] = v;
-                    else if (g.dtype == F16) ((_Float16*)g.out)[at] = (_Float16)v;
-                    else ((__bf16*)g.out)[at] = (__bf16)v;
-                }
+                store_result(g.fin, b, bi, bj, lane, acc[i][j], c2);
             } else {
                 half4 am_hi[4], am_lo[4];
                 if constexpr (MODE == POLY) {
@@ -495,6 +507,237 @@ __global__ __launch_bounds__(C::NW * 64) void k_ns_gemm(const NsGemm g) {
                 }
             }
         }
+}
+
+// ---- a whole matrix in one workgroup and one launch ----------------------------------------------------------------------------------------
+// Small matrices are bound by launches: 17 of them take 70 us of GPU or 100 us of host time whatever the size.  Here one workgroup of 16 waves
+// normalises, iterates and stores: A and M lie in LDS, X and X^T too where they fit (LOCAL; else in the workspace: the CU's own writes and reads).
+// MB = 32-row blocks of X; Gram's K is shared out to G = 16 / MB^2 groups of waves and added up in LDS.  A wave takes 32 columns of X from X^T, and
+// writes them back in place: nobody else reads them before the barrier.
+struct OneArgs {
+    const void* in; View iv;
+    int rows, cols;
+    _Float16 *x, *xt;                        // per matrix 32 MB x np x P halfs each
+    int np;                                  // columns, padded to 32
+    double eps;
+    int steps, dec;
+    float c0, c1, c2, scale;
+    MuonArgs mu;
+    Output fin;
+};
+constexpr int one_groups(int mb) { return 16 / (mb * mb); }
+// LDS: A, M, partial Gram tiles; X and X^T for LOCAL
+constexpr int one_lds(int mb, int p, int np) { return 2 * mb * 2 * mb * p * 1024 + (one_groups(mb) - 1) * mb * mb * 4096 + 2 * 32 * mb * np * p * 2; }
+
+template <int P>
+__device__ __forceinline__ void split(const f32x16& v, half4 (&hi)[4], half4 (&lo)[4]) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        const float x = one_value(v[r]);
+        hi[r >> 2][r & 3] = (_Float16)x;
+        if (P == 2) lo[r >> 2][r & 3] = (_Float16)(x - (float)hi[r >> 2][r & 3]);
+    }
+}
+template <int P>
+__device__ __forceinline__ void mfma_split(const half8 (&a)[P], const half8 (&b)[P], f32x16& acc) {
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], b[0], acc, 0, 0, 0);
+    if constexpr (P == 2) {
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[1], b[0], acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], b[1], acc, 0, 0, 0);
+    }
+}
+
+template <int T, bool MUON, int P, int MB, bool LOCAL>
+__global__ __launch_bounds__(1024) void k_ns_one(const OneArgs g) {
+    typedef typename Elem<T>::type E;
+    constexpr int WAVES = 16, KM = 2 * MB, G = one_groups(MB), AH = MB * KM * P * 512;       // k steps of A; groups; halfs of A
+    extern __shared__ __attribute__((aligned(1024))) char smem[];
+    _Float16 *la = (_Float16*)smem, *lm = la + AH;               // A, M in fragment order
+    f32x4* red = (f32x4*)(lm + AH);                              // partial Gram tiles of groups 1 .. G - 1
+    __shared__ double sums[WAVES];
+    const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const E* src = (const E*)g.in + b * g.iv.bs;
+    float* mom = MUON ? g.mu.mom + b * g.mu.mv.bs : nullptr;
+    const float gs = MUON ? (g.mu.gscale_dev ? *g.mu.gscale_dev : g.mu.gscale) : 1.f;
+    // ---- norm, and the momentum update ----
+    double s = 0.0;
+    {
+        const unsigned cols = g.cols, n = (unsigned)g.rows * cols;
+        for (unsigned i0 = tid; i0 < n; i0 += 4 * WAVES * 64) {
+            float v[4], m[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const unsigned i = i0 + WAVES * 64 * k, r = i / cols, c = i - r * cols;
+                v[k] = i < n ? (float)src[r * g.iv.ld + c] : 0.f;
+                if (MUON) m[k] = i < n ? mom[r * g.mu.mv.ld + c] : 0.f;
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const unsigned i = i0 + WAVES * 64 * k, r = i / cols, c = i - r * cols;
+                if (MUON && i < n) {
+                    v[k] *= gs;
+                    m[k] = muon_mom(g.mu, v[k], m[k]);
+                    mom[r * g.mu.mv.ld + c] = m[k];
+                    v[k] = muon_u(g.mu, v[k], m[k]);
+                }
+                s = fma((double)v[k], (double)v[k], s);
+            }
+        }
+    }
+    for (int k = 32; k > 0; k >>= 1) s += __shfl_xor(s, k);
+    if (lane == 0) sums[wave] = s;
+    __syncthreads();
+    s = 0.0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) s += sums[w];
+    const double norm = sqrt(s), t = norm / (norm + g.eps);
+    int e0 = 0;
+    if (t < 0.5) e0 = t > 1e-18 ? -ilogb(t) - 1 : 59;            // (as k_ns_prep)
+    const double f = ldexp((double)X_SCALE, e0) / (norm + g.eps);
+    // ---- normalised fragments of X and X^T ----
+    const int nk = g.np >> 4, jb = g.np >> 5;                    // k steps and 32-column blocks of X
+    const long long xs = (long long)32 * MB * g.np * P;
+    _Float16 *x, *xt;
+    if constexpr (LOCAL) { x = (_Float16*)(red + (G - 1) * MB * MB * 256); xt = x + 32 * MB * g.np * P; }
+    else { x = g.x + b * xs; xt = g.xt + b * xs; }
+    for (int q = wave; q < 2 * MB * nk; q += WAVES) {
+        const bool tr = q >= MB * nk;
+        const int z = tr ? q - MB * nk : q, blk = tr ? z / KM : z / nk, k16 = tr ? z - blk * KM : z - blk * nk;
+        half8 hi, lo;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int p0 = 32 * blk + (lane & 31), p1 = 16 * k16 + 8 * (lane >> 5) + e;       // (row, column) of X, or (column, row)
+            const int r = tr == (g.fin.tall != 0) ? p0 : p1, c = tr == (g.fin.tall != 0) ? p1 : p0;
+            float v = 0.f;
+            if (r < g.rows && c < g.cols) {
+                v = (float)src[r * g.iv.ld + c];
+                if (MUON) v = muon_u(g.mu, v * gs, mom[r * g.mu.mv.ld + c]);
+                v = (float)((double)v * f);
+            }
+            v = one_value(v);
+            hi[e] = (_Float16)v;
+            lo[e] = (_Float16)(v - (float)hi[e]);
+        }
+        _Float16* d = (tr ? xt + ((long long)blk * KM + k16) * P * 512 : x + ((long long)blk * nk + k16) * P * 512) + lane * 8;
+        *(half8*)d = hi;
+        if (P == 2) *(half8*)(d + 512) = lo;
+    }
+    __syncthreads();
+    half8 ident[2];
+#pragma unroll
+    for (int pi = 0; pi < 2; ++pi)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ident[pi][e] = (lane & 31) == 16 * pi + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3) ? (_Float16)1.f : (_Float16)0.f;
+    const int grp = wave / (MB * MB), tile = wave % (MB * MB), bi = tile / MB, bj = tile % MB, used = nk < G ? nk : G;      // groups with a k step
+    for (int step = 0; step < g.steps; ++step) {
+        const int ek = max(0, e0 - step * g.dec), ek1 = max(0, e0 - (step + 1) * g.dec);
+        half4 hi[4], lo[4];
+        f32x16 acc;
+        // ---- A = X X^T ----
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[r] = 0.f;
+        {
+            const _Float16 *pa = x + (long long)bi * nk * P * 512 + lane * 8, *pb = x + (long long)bj * nk * P * 512 + lane * 8;
+            constexpr int R = 4;                                 // k steps in flight
+            for (int k0 = grp; k0 < nk; k0 += R * G) {
+                half8 fa[R][P], fb[R][P];
+#pragma unroll
+                for (int u = 0; u < R; ++u) {
+                    const int k = k0 + u * G < nk ? k0 + u * G : k0;
+#pragma unroll
+                    for (int p = 0; p < P; ++p) {
+                        fa[u][p] = *(const half8*)(pa + ((long long)k * P + p) * 512);
+                        fb[u][p] = *(const half8*)(pb + ((long long)k * P + p) * 512);
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < R; ++u)
+                    if (k0 + u * G < nk) mfma_split<P>(fa[u], fb[u], acc);
+            }
+        }
+        if (grp > 0 && grp < used) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) red[((grp - 1) * MB * MB + tile) * 256 + q * 64 + lane] = f32x4{acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
+        }
+        __syncthreads();
+        if (grp == 0) {
+#pragma unroll 3
+            for (int z = 0; z < used - 1; ++z)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const f32x4 v = red[(z * MB * MB + tile) * 256 + q * 64 + lane];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[4 * q + e] += v[e];
+                }
+            const float c = ldexpf(A_SCALE / (X_SCALE * X_SCALE), -2 * ek);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[r] *= c;
+            split<P>(acc, hi, lo);
+            store_frag<P>(la, KM, bj, 2 * bi, lane, hi, lo);
+        }
+        __syncthreads();
+        // ---- M = c0 I + c1 A + c2 A A ----
+        if (grp == 0) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[r] = 0.f;
+#pragma unroll
+            for (int k = 0; k < KM; ++k) {
+                half8 fa[P], fb[P];
+#pragma unroll
+                for (int p = 0; p < P; ++p) {
+                    fa[p] = *(const half8*)(la + ((bi * KM + k) * P + p) * 512 + lane * 8);
+                    fb[p] = *(const half8*)(la + ((bj * KM + k) * P + p) * 512 + lane * 8);
+                }
+                mfma_split<P>(fa, fb, acc);
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int q = r >> 2, d = ((bj * KM + 2 * bi + (q >> 1)) * P) * 512 + ((lane & 31) + 32 * (q & 1)) * 8 + 4 * (lane >> 5) + (r & 3);
+                float am = (float)la[d];
+                if (P == 2) am += (float)la[d + 512];
+                acc[r] = fmaf(g.c1, am, acc[r] * g.c2);
+                if (bi == bj && 8 * q + 4 * (lane >> 5) + (r & 3) == (lane & 31)) acc[r] += g.c0;
+            }
+            split<P>(acc, hi, lo);
+            store_frag<P>(lm, KM, bj, 2 * bi, lane, hi, lo);
+        }
+        __syncthreads();
+        // ---- X <- M X: a wave takes 32 columns at a time ----
+        const bool last = step + 1 == g.steps;
+        const float c = last ? ldexpf(g.scale / (A_SCALE * X_SCALE), -ek) : ldexpf(1.f / A_SCALE, ek1 - ek);
+        for (int j = wave; j < jb; j += WAVES) {
+            half8 fb[KM][P];
+#pragma unroll
+            for (int k = 0; k < KM; ++k)
+#pragma unroll
+                for (int p = 0; p < P; ++p) fb[k][p] = *(const half8*)(xt + (((long long)j * KM + k) * P + p) * 512 + lane * 8);
+#pragma unroll 1
+            for (int i = 0; i < MB; ++i) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[r] = 0.f;
+#pragma unroll
+                for (int k = 0; k < KM; ++k) {
+                    half8 fa[P];
+#pragma unroll
+                    for (int p = 0; p < P; ++p) fa[p] = *(const half8*)(lm + ((i * KM + k) * P + p) * 512 + lane * 8);
+                    mfma_split<P>(fa, fb[k], acc);
+                }
+                if (last) {
+                    store_result(g.fin, b, i, j, lane, acc, c);
+                    continue;
+                }
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[r] *= c;
+                split<P>(acc, hi, lo);
+                store_frag<P>(xt, KM, j, 2 * i, lane, hi, lo);
+                half4 th[4], tl[4];
+                transpose_tile(hi, ident, th);
+                if (P == 2) transpose_tile(lo, ident, tl);
+                store_frag<P>(x, nk, i, 2 * j, lane, th, tl);
+            }
+        }
+        __syncthreads();
+    }
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------------------------
@@ -569,6 +812,7 @@ int gemm(NsGemm& g, const Cut& c, hipStream_t st) {
 
 struct Plan {
     int P, m, n, mp, np, tall, n_part, dec;
+    int one, local;                          // 32-row blocks of X where one workgroup takes a matrix (k_ns_one), else 0; with X in LDS
     Cut gram, poly, full;
     long long off_part, off_sc, off_count, n_count, off_split, off_x, off_xt[2], off_a, off_m, bytes;
 };
@@ -613,6 +857,20 @@ int make_plan(const dsvc_ortho_cfg* c, Plan* p) {
     p->m = p->tall ? c->cols : c->rows;
     p->n = p->tall ? c->rows : c->cols;
     if (!c->batch || !p->m) return DSVC_OK;
+    long long at = 0;
+    auto take = [&](long long bytes) { const long long o = at; at += (bytes + 1023) / 1024 * 1024; return o; };
+    const int mb = p->m <= 32 ? 1 : 2;
+    if (p->m <= 64 && (long long)32 * mb * p->n <= ONE_WORK) {
+        p->one = mb;
+        p->mp = 32 * mb;
+        p->np = round_up(p->n, 32);
+        p->local = one_lds(mb, p->P, p->np) <= ONE_LDS;
+        const long long xs = p->local ? 0 : (long long)c->batch * p->mp * p->np * p->P * 2;
+        p->off_x = take(xs);
+        p->off_xt[0] = take(xs);
+        p->bytes = at ? at : 256;
+        return DSVC_OK;
+    }
     p->mp = round_up(p->m, PAD);
     p->np = round_up(p->n, PAD);
     if ((long long)c->batch * (p->mp / 64) * (p->np / 64) >= (1LL << 22)) return fail(DSVC_EINVAL, "orthogonalize: shape [%d, %d, %d] is too large", c->batch, c->rows, c->cols);
@@ -627,8 +885,6 @@ int make_plan(const dsvc_ortho_cfg* c, Plan* p) {
     }
     const long long want = ((long long)p->m * p->n + 8191) / 8192;
     p->n_part = (int)(want < SUM_BLOCKS ? want : SUM_BLOCKS);
-    long long at = 0;
-    auto take = [&](long long bytes) { const long long o = at; at += (bytes + 1023) / 1024 * 1024; return o; };
     const long long B = c->batch, xs = B * p->mp * p->np * p->P * 2, as = B * p->mp * p->mp * p->P * 2;
     p->off_part = take(B * p->n_part * 8);
     p->off_sc = take(B * (long long)sizeof(Scalars));
@@ -646,6 +902,22 @@ int make_plan(const dsvc_ortho_cfg* c, Plan* p) {
     p->off_m = take(as);
     p->bytes = at;
     return DSVC_OK;
+}
+
+template <int T, bool MUON, int P, int MB, bool LOCAL>
+int one_mb(const OneArgs& g, int batch, hipStream_t st) {
+    const int lds = one_lds(MB, P, LOCAL ? g.np : 0);
+    if (lds > 64 * 1024) DSVC_HIP(hipFuncSetAttribute((const void*)k_ns_one<T, MUON, P, MB, LOCAL>, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+    hipLaunchKernelGGL((k_ns_one<T, MUON, P, MB, LOCAL>), dim3(batch), dim3(1024), lds, st, g);
+    DSVC_HIP(hipGetLastError());
+    return DSVC_OK;
+}
+template <int T, bool MUON, int P>
+int one(const dsvc_ortho_cfg* c, const Plan& p, const void* in, View iv, void* out, View ov, const MuonArgs& mu, char* ws, hipStream_t st) {
+    const OneArgs g{in, iv, c->rows, c->cols, (_Float16*)(ws + p.off_x), (_Float16*)(ws + p.off_xt[0]), p.np, (double)c->eps, c->steps, p.dec,
+                    c->coef[0] * A_SCALE, c->coef[1], c->coef[2] / A_SCALE, c->scale, mu, Output{out, ov, c->dtype, p.m, p.n, p.tall, mu}};
+    if (p.one == 1) return p.local ? one_mb<T, MUON, P, 1, true>(g, c->batch, st) : one_mb<T, MUON, P, 1, false>(g, c->batch, st);
+    return p.local ? one_mb<T, MUON, P, 2, true>(g, c->batch, st) : one_mb<T, MUON, P, 2, false>(g, c->batch, st);
 }
 
 template <int T, bool MUON, int P>
@@ -667,13 +939,6 @@ int prep(const dsvc_ortho_cfg* c, const Plan& p, const void* in, View iv, const 
                        (Scalars*)(ws + p.off_sc));
     DSVC_HIP(hipGetLastError());
     return DSVC_OK;
-}
-
-template <bool MUON, int P>
-int prep_t(const dsvc_ortho_cfg* c, const Plan& p, const void* in, View iv, const MuonArgs& mu, char* ws, hipStream_t st) {
-    if (c->dtype == F32) return prep<F32, MUON, P>(c, p, in, iv, mu, ws, st);
-    if (c->dtype == F16) return prep<F16, MUON, P>(c, p, in, iv, mu, ws, st);
-    return prep<BF16, MUON, P>(c, p, in, iv, mu, ws, st);
 }
 
 template <int P>
@@ -698,10 +963,24 @@ int iterate(const dsvc_ortho_cfg* c, const Plan& p, void* out, View ov, const Mu
         g.c2 = 1.f / A_SCALE;
         if (k + 1 < c->steps) { DSVC_TRY((gemm<P, FULL>(g, p.full, st))); continue; }
         g.c2 = c->scale / (A_SCALE * X_SCALE);
-        g.out = out; g.ov = ov; g.dtype = c->dtype; g.m = p.m; g.n = p.n; g.tall = p.tall; g.mu = mu;
+        g.fin = Output{out, ov, c->dtype, p.m, p.n, p.tall, mu};
         DSVC_TRY((gemm<P, FINAL>(g, p.full, st)));
     }
     return DSVC_OK;
+}
+
+// the whole operator on the workspace's plan
+template <int T, bool MUON, int P>
+int run_t(const dsvc_ortho_cfg* c, const Plan& p, const void* in, View iv, void* out, View ov, const MuonArgs& mu, char* ws, hipStream_t st) {
+    if (p.one) return one<T, MUON, P>(c, p, in, iv, out, ov, mu, ws, st);
+    DSVC_TRY((prep<T, MUON, P>(c, p, in, iv, mu, ws, st)));
+    return iterate<P>(c, p, out, ov, mu, ws, st);
+}
+template <bool MUON>
+int run(const dsvc_ortho_cfg* c, const Plan& p, const void* in, View iv, void* out, View ov, const MuonArgs& mu, char* ws, hipStream_t st) {
+    if (c->dtype == F32) return p.P == 2 ? run_t<F32, MUON, 2>(c, p, in, iv, out, ov, mu, ws, st) : run_t<F32, MUON, 1>(c, p, in, iv, out, ov, mu, ws, st);
+    if (c->dtype == F16) return p.P == 2 ? run_t<F16, MUON, 2>(c, p, in, iv, out, ov, mu, ws, st) : run_t<F16, MUON, 1>(c, p, in, iv, out, ov, mu, ws, st);
+    return p.P == 2 ? run_t<BF16, MUON, 2>(c, p, in, iv, out, ov, mu, ws, st) : run_t<BF16, MUON, 1>(c, p, in, iv, out, ov, mu, ws, st);
 }
 
 int check_view(const char* what, int64_t ld, int64_t bs, int rows, int cols, int batch, bool written) {
@@ -732,16 +1011,7 @@ int dsvc_orthogonalize(const dsvc_ortho_cfg* c, const void* in, int64_t in_ld, i
     if (workspace_bytes < p.bytes || (uintptr_t)workspace % 256) return fail(DSVC_EINVAL, "orthogonalize: workspace of %lld bytes at %p, need %lld on 256", (long long)workspace_bytes, workspace, p.bytes);
     DSVC_TRY(check_view("input", in_ld, in_bs, c->rows, c->cols, c->batch, false));
     DSVC_TRY(check_view("output", out_ld, out_bs, c->rows, c->cols, c->batch, true));
-    char* ws = (char*)workspace;
-    hipStream_t st = (hipStream_t)stream;
-    const MuonArgs none{};
-    const View iv{in_ld, in_bs}, ov{out_ld, out_bs};
-    if (p.P == 2) {
-        DSVC_TRY((prep_t<false, 2>(c, p, in, iv, none, ws, st)));
-        return iterate<2>(c, p, out, ov, none, ws, st);
-    }
-    DSVC_TRY((prep_t<false, 1>(c, p, in, iv, none, ws, st)));
-    return iterate<1>(c, p, out, ov, none, ws, st);
+    return run<false>(c, p, in, View{in_ld, in_bs}, out, View{out_ld, out_bs}, MuonArgs{}, (char*)workspace, (hipStream_t)stream);
 }
 
 int dsvc_muon_step(const dsvc_ortho_cfg* c, void* param, int64_t param_ld, int64_t param_bs, const void* grad, int64_t grad_ld, int64_t grad_bs, float* momentum,
@@ -756,16 +1026,8 @@ int dsvc_muon_step(const dsvc_ortho_cfg* c, void* param, int64_t param_ld, int64
     DSVC_TRY(check_view("parameter", param_ld, param_bs, c->rows, c->cols, c->batch, true));
     DSVC_TRY(check_view("gradient", grad_ld, grad_bs, c->rows, c->cols, c->batch, false));
     DSVC_TRY(check_view("momentum", mom_ld, mom_bs, c->rows, c->cols, c->batch, true));
-    char* ws = (char*)workspace;
-    hipStream_t st = (hipStream_t)stream;
     const MuonArgs u{momentum, View{mom_ld, mom_bs}, mu, lr, weight_decay, nesterov, grad_scale_dev, grad_scale};
-    const View gv{grad_ld, grad_bs}, pv{param_ld, param_bs};
-    if (p.P == 2) {
-        DSVC_TRY((prep_t<true, 2>(c, p, grad, gv, u, ws, st)));
-        return iterate<2>(c, p, param, pv, u, ws, st);
-    }
-    DSVC_TRY((prep_t<true, 1>(c, p, grad, gv, u, ws, st)));
-    return iterate<1>(c, p, param, pv, u, ws, st);
+    return run<true>(c, p, grad, View{grad_ld, grad_bs}, param, View{param_ld, param_bs}, u, (char*)workspace, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -26,13 +26,22 @@ def rms_scale(rows, cols, rms=0.2):
     return rms * math.sqrt(max(rows, cols))
 
 
+_coefficients = {}                 # (a, b, c) -> the C array
+
+
 def _cfg(t, steps, coefficients, eps, scale, precision):
-    if precision not in PLANES:
+    planes = PLANES.get(precision, -1)
+    if planes < 0:
         raise ValueError("precision must be one of %s, got %r" % ([k for k in PLANES if k], precision))
-    if len(coefficients) != 3:
-        raise ValueError("three coefficients, got %r" % (coefficients,))
+    coef = _coefficients.get(coefficients) if type(coefficients) is tuple else None
+    if coef is None:
+        if len(coefficients) != 3:
+            raise ValueError("three coefficients, got %r" % (coefficients,))
+        coef = (ctypes.c_float * 3)(*coefficients)
+        if type(coefficients) is tuple and len(_coefficients) < 64:
+            _coefficients[coefficients] = coef
     B, m, n = t.shape
-    return _lib.OrthoCfg(DTYPES[t.dtype], PLANES[precision], B, m, n, steps, (ctypes.c_float * 3)(*coefficients), eps, scale)
+    return _lib.OrthoCfg(DTYPES[t.dtype], planes, B, m, n, steps, coef, eps, scale)
 
 
 def _check(name, t):
@@ -47,24 +56,20 @@ def _check(name, t):
 def _matrices(name, t, copy):
     """t as [batch, rows, columns] with unit stride along the rows; ``copy``: in a new tensor where it does not lie so, else refused."""
     m, n = t.shape[-2:]
-    if t.dim() == 2:
-        v = t.unsqueeze(0)
-    elif t.dim() == 3:
-        v = t
-    else:
-        v = t.reshape(-1, m, n) if copy else t.view(-1, m, n)
-    ld, bs = v.stride(1), v.stride(0)
-    if (n <= 1 or v.stride(2) == 1) and (m <= 1 or ld >= n) and (v.shape[0] <= 1 or bs >= (m - 1) * ld + n):
+    d = t.dim()
+    v = t if d == 3 else t.unsqueeze(0) if d == 2 else t.reshape(-1, m, n) if copy else t.view(-1, m, n)
+    bs, ld, one = v.stride()
+    if (n <= 1 or one == 1) and (m <= 1 or ld >= n) and (v.shape[0] <= 1 or bs >= (m - 1) * ld + n):
         return v
     if copy:
         return v.contiguous()
     raise ValueError("%s is written in place: it needs rows of unit stride and matrices that do not overlap, got strides %s" % (name, t.stride()))
 
 
-def _workspace(cfg, device):
+def _workspace(L, cfg, t):
     need = ctypes.c_int64(0)
-    check(lib().dsvc_ortho_workspace(ctypes.byref(cfg), ctypes.byref(need)))
-    return torch.empty(need.value, device=device, dtype=torch.uint8)
+    check(L.dsvc_ortho_workspace(ctypes.byref(cfg), ctypes.byref(need)))
+    return torch.empty(need.value, device=t.device, dtype=torch.uint8), need.value
 
 
 @torch.no_grad()
@@ -73,16 +78,17 @@ def orthogonalize(x, steps=5, coefficients=COEFFICIENTS, eps=1e-7, scale=1.0, pr
     _check("x", x)
     v = _matrices("x", x, True)
     if out is None:
-        out = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+        out = x.new_empty(x.shape)
     elif out.shape != x.shape or out.dtype != x.dtype or out.device != x.device:
         raise ValueError("out must be %s %s on %s" % (tuple(x.shape), x.dtype, x.device))
     o = _matrices("out", out, False)
     cfg = _cfg(v, steps, coefficients, eps, scale, precision)
-    here, stream = on_device(x)
+    L = lib()
+    ws, size = _workspace(L, cfg, v)
+    here, stream = on_device(v)
     with here:
-        ws = _workspace(cfg, x.device)
-        check(lib().dsvc_orthogonalize(ctypes.byref(cfg), v.data_ptr(), v.stride(1), v.stride(0), o.data_ptr(), o.stride(1), o.stride(0), ws.data_ptr(),
-                                       ws.numel(), stream))
+        rc = L.dsvc_orthogonalize(ctypes.byref(cfg), v.data_ptr(), v.stride(1), v.stride(0), o.data_ptr(), o.stride(1), o.stride(0), ws.data_ptr(), size, stream)
+    check(rc)
     return out
 
 
@@ -109,9 +115,11 @@ def muon_step_(param, grad, momentum_buffer, lr, momentum=0.95, nesterov=True, w
         num_scale = float(grad_scale)
     p, g, m = _matrices("param", param, False), _matrices("grad", grad, True), _matrices("momentum_buffer", momentum_buffer, False)
     cfg = _cfg(p, steps, coefficients, eps, scale, precision)
-    here, stream = on_device(param)
+    L = lib()
+    ws, size = _workspace(L, cfg, p)
+    here, stream = on_device(p)
     with here:
-        ws = _workspace(cfg, param.device)
-        check(lib().dsvc_muon_step(ctypes.byref(cfg), p.data_ptr(), p.stride(1), p.stride(0), g.data_ptr(), g.stride(1), g.stride(0), m.data_ptr(), m.stride(1),
-                                   m.stride(0), lr, momentum, nesterov, weight_decay, dev_scale, num_scale, ws.data_ptr(), ws.numel(), stream))
+        rc = L.dsvc_muon_step(ctypes.byref(cfg), p.data_ptr(), p.stride(1), p.stride(0), g.data_ptr(), g.stride(1), g.stride(0), m.data_ptr(), m.stride(1),
+                              m.stride(0), lr, momentum, nesterov, weight_decay, dev_scale, num_scale, ws.data_ptr(), size, stream)
+    check(rc)
     return param
