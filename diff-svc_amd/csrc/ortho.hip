@@ -21,6 +21,8 @@
 // A and M are symmetric: only the tiles on and above the diagonal are computed, the mirrored tile is written by the same workgroup.
 #include <math.h>
 
+#include <utility>
+
 #include "../../include/dsvc.h"
 #include "common.h"
 
@@ -182,30 +184,76 @@ __global__ __launch_bounds__(256) void k_ns_prep(const void* __restrict__ in, Vi
 // ---- the products ----------------------------------------------------------------------------------------------------------------------
 enum { GRAM, POLY, FULL, FINAL };
 
-// the caller's tensor: the result, or (mu.mom) the parameter, out <- (1 - lr wd) out - lr result
+// the caller's tensor: the result, or (mu.mom) the parameter, out <- (1 - lr wd) out - lr result.  wide: neighbouring elements of a row may be accessed
+// as one (4 of a transposed result's, 2 of 16 bits of the other's)
 struct Output {
     void* out; View ov;
-    int dtype, m, n, tall;
+    int dtype, m, n, tall, wide;
     MuonArgs mu;
 };
-// 32 x 32 block (bi, bj) of matrix b, scaled by c: register r of a lane = row 8 (r >> 2) + 4 (lane >> 5) + (r & 3), column lane & 31
-__device__ __forceinline__ void store_result(const Output& o, int b, int bi, int bj, int lane, const f32x16& acc, float c) {
-    const int col = 32 * bj + (lane & 31);
+// 32 x 32 block (bi, bj) of matrix b, scaled by c: register r of a lane = row 8 (r >> 2) + 4 (lane >> 5) + (r & 3), column lane & 31.  Transposed, a lane has
+// four neighbours in memory; else neighbours are in neighbouring lanes, and pairs of 16-bit elements are put together by one exchange (element by
+// element a [768, 384] x 20 step's last product took 53 us, where the others take 25)
+template <class E>
+__device__ __forceinline__ void store_block(const Output& o, int b, int bi, int bj, int lane, const f32x16& acc, float c) {
+    typedef E E2 __attribute__((ext_vector_type(2)));
+    typedef E E4 __attribute__((ext_vector_type(4)));
+    E* out = (E*)o.out + b * o.ov.bs;
+    const int col = 32 * bj + (lane & 31), row0 = 32 * bi + 4 * (lane >> 5);
+    const bool step = o.mu.mom != nullptr;
+    const float keep = 1.f - o.mu.lr * o.mu.wd, lr = -o.mu.lr;
+    auto put = [&](E* p, float v) { *p = (E)(step ? fmaf(lr, v, keep * (float)*p) : v); };
+    if (o.tall) {
+        if (col >= o.n) return;
+        E* line = out + col * o.ov.ld;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int row = row0 + 8 * q;
+            if (o.wide && row + 3 < o.m) {
+                E4 v;
+                if (step) v = *(const E4*)(line + row);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = (E)(step ? fmaf(lr, acc[4 * q + e] * c, keep * (float)v[e]) : acc[4 * q + e] * c);
+                *(E4*)(line + row) = v;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (row + e < o.m) put(line + row + e, acc[4 * q + e] * c);
+            }
+        }
+        return;
+    }
+    if (sizeof(E) == 2 && o.wide) {
+        const bool odd = lane & 1;
+        const int c0 = col & ~1;             // the pair's columns: even lanes take a row's, odd lanes the next row's
+#pragma unroll
+        for (int r = 0; r < 16; r += 2) {
+            const float mine = (odd ? acc[r + 1] : acc[r]) * c, other = __shfl_xor((odd ? acc[r] : acc[r + 1]) * c, 1);
+            const int row = row0 + 8 * (r >> 2) + (r & 3) + odd;
+            if (row >= o.m || c0 >= o.n) continue;
+            E* p = out + row * o.ov.ld + c0;
+            const float a = odd ? other : mine, z = odd ? mine : other;
+            if (c0 + 1 < o.n) {
+                E2 v;
+                if (step) v = *(const E2*)p;
+                v[0] = (E)(step ? fmaf(lr, a, keep * (float)v[0]) : a);
+                v[1] = (E)(step ? fmaf(lr, z, keep * (float)v[1]) : z);
+                *(E2*)p = v;
+            } else put(p, a);
+        }
+        return;
+    }
     if (col >= o.n) return;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-        const int row = 32 * bi + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
-        if (row >= o.m) continue;
-        const long long at = b * o.ov.bs + (o.tall ? col * o.ov.ld + row : row * o.ov.ld + col);
-        float v = acc[r] * c;
-        if (o.mu.mom) {
-            const float p = o.dtype == F32 ? ((float*)o.out)[at] : o.dtype == F16 ? (float)((_Float16*)o.out)[at] : (float)((__bf16*)o.out)[at];
-            v = fmaf(-o.mu.lr, v, (1.f - o.mu.lr * o.mu.wd) * p);
-        }
-        if (o.dtype == F32) ((float*)o.out)[at] = v;
-        else if (o.dtype == F16) ((_Float16*)o.out)[at] = (_Float16)v;
-        else ((__bf16*)o.out)[at] = (__bf16)v;
+        const int row = row0 + 8 * (r >> 2) + (r & 3);
+        if (row < o.m) put(out + row * o.ov.ld + col, acc[r] * c);
     }
+}
+__device__ __forceinline__ void store_result(const Output& o, int b, int bi, int bj, int lane, const f32x16& acc, float c) {
+    if (o.dtype == F32) store_block<float>(o, b, bi, bj, lane, acc, c);
+    else if (o.dtype == F16) store_block<_Float16>(o, b, bi, bj, lane, acc, c);
+    else store_block<__bf16>(o, b, bi, bj, lane, acc, c);
 }
 
 struct NsGemm {
@@ -262,6 +310,9 @@ struct Tile {
     static constexpr int LDS = LDS_STAGES > LDS_JOIN ? LDS_STAGES : LDS_JOIN;
     static_assert(PIECES % NW == 0 && KS % G == 0 && PER * (NST - 2) < 64 && LDS * PER_CU <= 160 * 1024, "");
 };
+
+template <class F, int... I>
+__device__ __forceinline__ void each(F&& f, std::integer_sequence<int, I...>) { (f(std::integral_constant<int, I>{}), ...); }
 
 template <class C, int MODE>
 __global__ __launch_bounds__(C::NW * 64) void k_ns_gemm(const NsGemm g) {
@@ -460,6 +511,14 @@ __global__ __launch_bounds__(C::NW * 64) void k_ns_gemm(const NsGemm g) {
     if (MODE == GRAM) c2 = ldexpf(c2, -2 * ek);
     if (MODE == FULL) c2 = ldexpf(c2, ek1 - ek);
     if (MODE == FINAL) c2 = ldexpf(c2, -ek);
+    if constexpr (MODE == FINAL) {           // (not a loop: with this body hipcc keeps one, and the accumulators in scratch)
+        auto put = [&](auto ij) {
+            constexpr int i = decltype(ij)::value / TN, j = decltype(ij)::value % TN;
+            store_result(g.fin, b, ti * RA + wr * TM + i, tj * RB + wc * TN + j, lane, acc[i][j], c2);
+        };
+        each(put, std::make_integer_sequence<int, TM * TN>{});
+        return;
+    }
     half8 ident[2];
 #pragma unroll
     for (int pi = 0; pi < 2; ++pi)
@@ -470,9 +529,7 @@ __global__ __launch_bounds__(C::NW * 64) void k_ns_gemm(const NsGemm g) {
 #pragma unroll
         for (int j = 0; j < TN; ++j) {
             const int bi = ti * RA + wr * TM + i, bj = tj * RB + wc * TN + j;      // 32-blocks of the result
-            if constexpr (MODE == FINAL) {
-                store_result(g.fin, b, bi, bj, lane, acc[i][j], c2);
-            } else {
+            {
                 half4 am_hi[4], am_lo[4];
                 if constexpr (MODE == POLY) {
                     const _Float16* am = g.am + b * g.ot_bs;
@@ -904,6 +961,12 @@ int make_plan(const dsvc_ortho_cfg* c, Plan* p) {
     return DSVC_OK;
 }
 
+Output output(const dsvc_ortho_cfg* c, const Plan& p, void* out, View ov, const MuonArgs& mu) {
+    const int size = c->dtype == F32 ? 4 : 2, together = p.tall ? 4 : 2;
+    const bool wide = (uintptr_t)out % (size * together) == 0 && ov.ld % together == 0 && (c->batch == 1 || ov.bs % together == 0);
+    return Output{out, ov, c->dtype, p.m, p.n, p.tall, wide, mu};
+}
+
 template <int T, bool MUON, int P, int MB, bool LOCAL>
 int one_mb(const OneArgs& g, int batch, hipStream_t st) {
     const int lds = one_lds(MB, P, LOCAL ? g.np : 0);
@@ -915,7 +978,7 @@ int one_mb(const OneArgs& g, int batch, hipStream_t st) {
 template <int T, bool MUON, int P>
 int one(const dsvc_ortho_cfg* c, const Plan& p, const void* in, View iv, void* out, View ov, const MuonArgs& mu, char* ws, hipStream_t st) {
     const OneArgs g{in, iv, c->rows, c->cols, (_Float16*)(ws + p.off_x), (_Float16*)(ws + p.off_xt[0]), p.np, (double)c->eps, c->steps, p.dec,
-                    c->coef[0] * A_SCALE, c->coef[1], c->coef[2] / A_SCALE, c->scale, mu, Output{out, ov, c->dtype, p.m, p.n, p.tall, mu}};
+                    c->coef[0] * A_SCALE, c->coef[1], c->coef[2] / A_SCALE, c->scale, mu, output(c, p, out, ov, mu)};
     if (p.one == 1) return p.local ? one_mb<T, MUON, P, 1, true>(g, c->batch, st) : one_mb<T, MUON, P, 1, false>(g, c->batch, st);
     return p.local ? one_mb<T, MUON, P, 2, true>(g, c->batch, st) : one_mb<T, MUON, P, 2, false>(g, c->batch, st);
 }
@@ -963,7 +1026,7 @@ int iterate(const dsvc_ortho_cfg* c, const Plan& p, void* out, View ov, const Mu
         g.c2 = 1.f / A_SCALE;
         if (k + 1 < c->steps) { DSVC_TRY((gemm<P, FULL>(g, p.full, st))); continue; }
         g.c2 = c->scale / (A_SCALE * X_SCALE);
-        g.fin = Output{out, ov, c->dtype, p.m, p.n, p.tall, mu};
+        g.fin = output(c, p, out, ov, mu);
         DSVC_TRY((gemm<P, FINAL>(g, p.full, st)));
     }
     return DSVC_OK;
