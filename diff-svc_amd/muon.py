@@ -82,6 +82,8 @@ def orthogonalize(x, steps=5, coefficients=COEFFICIENTS, eps=1e-7, scale=1.0, pr
     elif out.shape != x.shape or out.dtype != x.dtype or out.device != x.device:
         raise ValueError("out must be %s %s on %s" % (tuple(x.shape), x.dtype, x.device))
     o = _matrices("out", out, False)
+    if out.untyped_storage().data_ptr() == v.untyped_storage().data_ptr() and (out.data_ptr() != v.data_ptr() or o.stride() != v.stride()):
+        v = v.clone()                  # shares memory, but not matrix by matrix: one may be written before another is read
     cfg = _cfg(v, steps, coefficients, eps, scale, precision)
     L = lib()
     ws, size = _workspace(L, cfg, v)
@@ -100,7 +102,8 @@ def muon_step_(param, grad, momentum_buffer, lr, momentum=0.95, nesterov=True, w
       g = grad * grad_scale;  m <- momentum m + (1 - momentum) g;  u = nesterov ? momentum m + (1 - momentum) g : m
       param <- (1 - lr weight_decay) param - lr * scale * orthogonalize(u)
 
-    momentum_buffer is float32; grad has param's type.  grad_scale: a number or a one-element float32 device tensor (a clip coefficient)."""
+    momentum_buffer is float32; grad has param's type; the three do not overlap.  grad_scale: a number or a one-element float32 device tensor (a
+    clip coefficient)."""
     _check("param", param)
     if grad.shape != param.shape or grad.dtype != param.dtype or grad.device != param.device:
         raise ValueError("grad must be %s %s on %s" % (tuple(param.shape), param.dtype, param.device))

@@ -144,18 +144,19 @@ class TokenEmbeddingHip(nn.Embedding):
                 raise NotImplementedError("TokenEmbeddingHip: %s" % k)
         super().__init__(num_embeddings, embedding_dim, padding_idx, **kw)
         self.scale = float(scale)
-        self._flag = None              # sticky device flag: a token outside the table (check)
+        # sticky flag: a token outside the table (check).  A buffer, so that it is there before a first call that is being captured into a graph
+        self.register_buffer("_flag", torch.zeros(1, dtype=torch.int32), persistent=False)
 
     def forward(self, tokens):
         if not self.weight.is_cuda:
             y = super().forward(tokens)
             return y * self.scale if self.scale != 1.0 else y
-        if self._flag is None or self._flag.device != self.weight.device:
+        if self._flag.device != self.weight.device:        # (a weight that was moved by itself)
             self._flag = torch.zeros(1, device=self.weight.device, dtype=torch.int32)
         return embed_tokens(tokens, self.weight, self.scale, self.padding_idx, self._flag)
 
     def check(self):
         """Raise IndexError if a lookup on the device since the last check was given a token outside the table.  Synchronises."""
-        if self._flag is not None and int(self._flag.item()):
+        if int(self._flag.item()):
             self._flag.zero_()
             raise IndexError("diffsvc_amd: a token lies outside [0, %d); its row was zero" % self.num_embeddings)

@@ -114,7 +114,8 @@ def test_orthogonalize(r, c, dtype, precision):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("shape, dtype", [((1100, 1300), torch.bfloat16), ((3, 512, 1024), torch.float32), ((2, 150, 4100), torch.float32), ((4100, 70), torch.float16),
-                                          ((24, 40, 30), torch.float32)])
+                                          ((24, 40, 30), torch.float32), ((300, 20, 31), torch.bfloat16), ((2, 64, 256), torch.float32), ((2, 65, 256), torch.float32),
+                                          ((33, 497), torch.float16), ((31, 512), torch.float32), ((513, 32), torch.float32)])
 def test_orthogonalize_larger(shape, dtype):
     g = update(shape, 77).to(dtype)
     close(M.orthogonalize(g.cuda()), g, dtype, 1 if dtype == torch.bfloat16 else 2)
@@ -166,6 +167,10 @@ def test_strides_and_in_place():
     assert torch.equal(buf[:, :, 30:230], want) and not buf[:, :, :30].any() and not buf[:, :, 230:].any()
     assert torch.equal(M.orthogonalize(buf.new_zeros(0, 3, 4)), buf.new_zeros(0, 3, 4))
     assert M.orthogonalize(buf.new_zeros(2, 0, 4)).shape == (2, 0, 4)
+    for shape in ((6, 20, 30), (6, 80, 90)):                               # one workgroup a matrix, and many
+        z = update((shape[0] + 1, *shape[1:]), 9).cuda()
+        want = M.orthogonalize(z[:-1].clone())
+        assert torch.equal(M.orthogonalize(z[:-1], out=z[1:]), want)      # the result of one matrix where the next one lies
     with pytest.raises(RuntimeError, match="singular values"):
         M.orthogonalize(buf, coefficients=(9.0, 9.0, 9.0))
     with pytest.raises(ValueError, match="in place"):
@@ -228,19 +233,21 @@ def test_streams_and_graph_replay():
     assert torch.equal(a, want) and torch.equal(b, want)
     p, m = update((2, 200, 300), 9, 1.0).cuda(), torch.zeros(2, 200, 300, device="cuda")
     pe, me = p.clone(), m.clone()
+    # (split along K, and small enough for one workgroup: their own counters and LDS on every replay)
+    wide, small = update((120, 3000), 10).cuda(), update((5, 20, 40), 11).cuda()
     graph, other = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
     M.muon_step_(p.clone(), g, m.clone(), 0.1)
     with torch.cuda.graph(graph):
         M.muon_step_(p, g, m, 0.1)
     with torch.cuda.graph(other, pool=graph.pool()):
-        o = M.orthogonalize(g)
+        o, ow, os = M.orthogonalize(g), M.orthogonalize(wide), M.orthogonalize(small)
     for k in range(4):
         g.copy_(update((2, 200, 300), 20 + k))
         graph.replay()
         M.muon_step_(pe, g, me, 0.1)
         assert torch.equal(p, pe) and torch.equal(m, me), k
         other.replay()
-        assert torch.equal(o, M.orthogonalize(g))
+        assert torch.equal(o, M.orthogonalize(g)) and torch.equal(ow, M.orthogonalize(wide)) and torch.equal(os, M.orthogonalize(small))
         torch.cuda.synchronize()
 
 

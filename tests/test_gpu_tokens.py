@@ -194,3 +194,51 @@ def test_streams_and_graph_replay():
         e = T.embed_tokens_grad(t, dy, V, padding_idx=0)
         assert torch.equal(wg, e) and torch.equal(yg, e[t] * 0.5), k
         torch.cuda.synchronize()
+
+
+def test_offsets_beyond_32_bits():
+    """A table of 2^31 + elements (rows and gradients at its end)."""
+    V, H = (1 << 20) + 7, 2056
+    w = torch.empty(V, H, device="cuda", dtype=torch.bfloat16)
+    w[-9:] = torch.arange(9, device="cuda", dtype=torch.bfloat16)[:, None] + 1
+    w[:3] = 0.5
+    t = torch.tensor([V - 1, 0, V - 9, 2, V - 1], device="cuda")
+    y = T.embed_tokens(t, w, 2.0)
+    assert torch.equal(y[:, 0].float().cpu(), torch.tensor([18.0, 1, 2, 1, 18])) and bool((y == y[:, :1]).all())
+    del w
+    g = T.embed_tokens_grad(t, y, V)
+    assert torch.equal(g[-1].float(), torch.full((H,), 36.0, device="cuda")) and torch.equal(g[V - 9], y[2]) and torch.equal(g[2], y[3])
+    assert not g[3:V - 9].any() and not g[V - 8:V - 1].any()
+
+
+def test_module_captured_with_its_backward_pass():
+    """A first call of the module inside a capture, gradient and all, replayed on new tokens; its flag is not the graph's memory."""
+    torch.manual_seed(0)
+    m = T.TokenEmbeddingHip(40, 16, padding_idx=0, scale=0.5).cuda()
+    t, r = torch.randint(0, 40, (500,), device="cuda"), torch.randn(500, 16, device="cuda")
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):                             # (autograd's own first-use work happens outside the capture)
+        torch.autograd.grad((T.embed_tokens(t, m.weight) * r).sum(), m.weight)
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = m(t)
+        dw, = torch.autograd.grad(y, m.weight, r)
+    for k in range(4):
+        t.copy_(torch.randint(0, 40, (500,), device="cuda"))
+        r.copy_(torch.randn(500, 16, device="cuda"))
+        graph.replay()
+        with torch.no_grad():
+            assert torch.equal(y.detach(), m.weight[t] * 0.5), k
+        assert torch.equal(dw, T.embed_tokens_grad(t, r, 40, 0.5, 0)), k
+        torch.cuda.synchronize()
+    m.check()
+    t[3] = 40
+    graph.replay()
+    with pytest.raises(IndexError):
+        m.check()
+    graph.replay()
+    with pytest.raises(IndexError):
+        m.check()
+    assert list(m.state_dict()) == ["weight"]
