@@ -5,9 +5,10 @@
 //   steps times:  A = X X^T,  M = a I + b A + c A A,  X <- M X            (the singular values go through s (a + b s^2 + c s^4))
 //   O = scale * X                (transposed back)
 //
-// Arithmetic: every product is an fp16 MFMA (v_mfma_f32_32x32x16_f16) with fp32 accumulation.  bf16 tensors run on ONE fp16 plane (its 11 bits stay
-// below the 8 of the result: 1.2e-3 against a half step of 1.7e-3 rms); fp32 and fp16 tensors on hi + lo planes and three MFMAs per product
-// (hi hi + hi lo + lo hi: 22 bits per operand, fp32-class, the trainer's own scheme).
+// Arithmetic: every product is an fp16 MFMA (v_mfma_f32_32x32x16_f16) with fp32 accumulation.  Large bf16 tensors run on ONE fp16 plane (its 11 bits stay
+// below the 8 of the result: 1.2e-3 against a half step of 1.7e-3 rms); the rest on hi + lo planes and three MFMAs per product (hi hi + hi lo +
+// lo hi: 22 bits per operand, fp32-class, the trainer's own scheme).  Small bf16 tensors too: launches bound them, not products, and the
+// roundings of few elements do not average (2.9e-3 on one plane at [8, 24]).
 // The planes hold X * 2^12 and A, M * 2^10: |X| and |M| are bounded by the polynomial on [0, 1] (checked on the host for the caller's
 // coefficients), so fp16's top is out of reach and small elements keep their bits; an update whose norm eps swamps is carried with an
 // extra power of two that shrinks as the iterate grows (Scalars::e0).  Norms are summed in fp64: no square of a tiny gradient underflows.
@@ -41,6 +42,7 @@ constexpr int PAD = 128;                     // rows and columns of every interm
 // Padded elements up to which one workgroup takes a matrix of up to 64 rows.  fp32, one workgroup against 17 launches (GPU time; the host takes 70 us to
 // launch them): [1, 1] 24 / 71 us, [64, 64] x 8 27 / 76, [64, 256] 52 / 80, [32, 500] 72 / 88, [64, 1024] 163 / 103; [48, 64] x 2000 197 / 1162
 constexpr long long ONE_WORK = 16384;
+constexpr double ONE_PLANE = 1 << 27;        // multiply-adds of a product of the batch from which bf16 takes one plane
 constexpr int ONE_LDS = 156 * 1024;          // its LDS (the rest: static)
 constexpr int SUM_BLOCKS = 256;              // partial sums of squares per matrix
 
@@ -798,30 +800,35 @@ __global__ __launch_bounds__(1024) void k_ns_one(const OneArgs g) {
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------------------------
-// Tiles.  128: 64 x 64 per wave (4 or 8 fragment reads feed 4 or 12 MFMAs), two workgroups a CU hide each other's barriers; stages of 64 (one plane) or
-// 32 (two) k.  256: 128 x 64 per wave, fewer LDS reads per MFMA.  64: a wave has one accumulator tile, four stages ahead; for grids that 128 leaves
-// mostly empty.
+// Tiles.  128: 64 x 64 per wave (4 or 8 fragment reads feed 4 or 12 MFMAs), two workgroups a CU hide each other's barriers; four stages of 16 k at two
+// planes (against two of 32: [768, 384] x 20 fp32 272 -> 253 us, [768, 1152] x 20 1055 -> 1031, [4096, 4096] 4.01 -> 4.10 ms), two of 64 at one.  ALONE: the
+// same tile by eight waves, where there is about one to a CU ([2048, 2048] fp32: 757 -> 690 us, [1000, 3000] 362 -> 334).  256: 128 x 64 per wave, fewer LDS
+// reads per MFMA.  64: a wave has one accumulator tile, four stages ahead; for grids that 128 leaves mostly empty.
+constexpr int ALONE = 129;                   // a tile of 128 with a CU to itself
 template <int P, int SIZE> struct Tiles;
 template <> struct Tiles<1, 64> { typedef Tile<1, 1, 1, 2, 2, 1, 4, 4, 2> type; };
 template <> struct Tiles<2, 64> { typedef Tile<2, 1, 1, 2, 2, 1, 2, 4, 2> type; };
 template <> struct Tiles<1, 128> { typedef Tile<1, 2, 2, 2, 2, 1, 4, 2, 2> type; };
-template <> struct Tiles<2, 128> { typedef Tile<2, 2, 2, 2, 2, 1, 2, 2, 2> type; };
+template <> struct Tiles<2, 128> { typedef Tile<2, 2, 2, 2, 2, 1, 1, 4, 2> type; };
+template <> struct Tiles<1, ALONE> { typedef Tile<1, 1, 2, 4, 2, 1, 8, 2, 1> type; };
+template <> struct Tiles<2, ALONE> { typedef Tile<2, 1, 2, 4, 2, 1, 4, 2, 1> type; };
 template <> struct Tiles<1, 256> { typedef Tile<1, 4, 2, 2, 4, 1, 4, 2, 1> type; };
 
 constexpr int CUS = 256;
 
 // How one product is cut: the tile's edge, and which tiles are split along K.
 struct Cut {
-    int size, tiles_i, n_tiles, full, rest, slices;
+    int kind, size, tiles_i, n_tiles, full, rest, slices;
     long long part_bytes() const { return slices > 1 ? (long long)rest * slices * size * size * 4 : 0; }
 };
 // A slice keeps at least 16 stages: a partial tile's way through memory costs about as much as 8 ([4, 1024, 1024] bf16: 253 us whole, 344 us in slices of
 // 8 or more; [100, 4000] fp32: 250 us whole, 124 us in slices of 16; the last 16 of [4096, 4096] bf16's 528 tiles: 1783 -> 1638 us).
 constexpr int MIN_STAGES = 16;
 template <class C>
-Cut cut_for(int size, bool sym, int batch, int mi, int nj, int k16) {
+Cut cut_for(int kind, bool sym, int batch, int mi, int nj, int k16) {
+    const int size = 32 * C::TM * C::WR;
     Cut c{};
-    c.size = size;
+    c.kind = kind; c.size = size;
     c.tiles_i = mi / size;
     c.n_tiles = sym ? c.tiles_i * (c.tiles_i + 1) / 2 : c.tiles_i * (nj / size);
     const long long total = (long long)batch * c.n_tiles, slots = C::PER_CU * CUS;
@@ -838,13 +845,14 @@ Cut cut_for(int size, bool sym, int batch, int mi, int nj, int k16) {
 }
 template <int P>
 Cut cut(bool sym, int batch, int mi, int nj, int k16) {
-    // 128 where that gives every CU a tile ([1000, 3000] fp32 on 36 ... 192 tiles of 128: 665 us, on tiles of 64: 376 us; [768, 384] x 20: 346 -> 282 us;
-    // [2048, 2048]'s symmetric products on 136 tiles in K slices: 869 us, on tiles of 64: 781 us).  256 where it still gives one to each and nothing is
-    // padded for it ([4096, 4096] bf16, the full product: 158 -> 140 us)
+    // 128 where that gives about every CU a tile ([1000, 3000] fp32 on 36 ... 192 tiles of 128 by four waves: 665 us, on tiles of 64: 376 us; [2048, 2048]'s
+    // symmetric products on 136 tiles in K slices: 869 us, on tiles of 64: 781 us).  256 where it still gives one to each and nothing is padded for it
+    // ([4096, 4096] bf16, the full product: 158 -> 140 us)
     const int t = mi / 128;
     const long long tiles = (long long)batch * (sym ? t * (t + 1) / 2 : (long long)t * (nj / 128));
     if (P == 1 && !sym && mi % 256 == 0 && nj % 256 == 0 && tiles >= 4 * CUS) return cut_for<typename Tiles<1, 256>::type>(256, sym, batch, mi, nj, k16);
-    if (tiles >= CUS) return cut_for<typename Tiles<P, 128>::type>(128, sym, batch, mi, nj, k16);
+    if (tiles > CUS) return cut_for<typename Tiles<P, 128>::type>(128, sym, batch, mi, nj, k16);
+    if (tiles >= CUS * 3 / 4) return cut_for<typename Tiles<P, ALONE>::type>(ALONE, sym, batch, mi, nj, k16);
     return cut_for<typename Tiles<P, 64>::type>(64, sym, batch, mi, nj, k16);
 }
 
@@ -861,9 +869,10 @@ template <int P, int MODE>
 int gemm(NsGemm& g, const Cut& c, hipStream_t st) {
     g.tiles_i = c.tiles_i; g.n_tiles = c.n_tiles; g.full = c.full; g.rest = c.rest; g.slices = c.slices;
     if constexpr (P == 1 && (MODE == FULL || MODE == FINAL)) {
-        if (c.size == 256) return launch_gemm<typename Tiles<1, 256>::type, MODE>(g, st);
+        if (c.kind == 256) return launch_gemm<typename Tiles<1, 256>::type, MODE>(g, st);
     }
-    if (c.size == 128) return launch_gemm<typename Tiles<P, 128>::type, MODE>(g, st);
+    if (c.kind == 128) return launch_gemm<typename Tiles<P, 128>::type, MODE>(g, st);
+    if (c.kind == ALONE) return launch_gemm<typename Tiles<P, ALONE>::type, MODE>(g, st);
     return launch_gemm<typename Tiles<P, 64>::type, MODE>(g, st);
 }
 
@@ -909,10 +918,10 @@ int make_plan(const dsvc_ortho_cfg* c, Plan* p) {
     DSVC_TRY(check_coefficients(c->coef, c->steps, &growth));
     *p = Plan{};
     p->dec = growth > 1.0 ? (int)ceil(log2(growth) + 1e-6) : 0;
-    p->P = c->planes ? c->planes : c->dtype == BF16 ? 1 : 2;
     p->tall = c->rows > c->cols;
     p->m = p->tall ? c->cols : c->rows;
     p->n = p->tall ? c->rows : c->cols;
+    p->P = c->planes ? c->planes : c->dtype == BF16 && (double)c->batch * p->m * p->m * p->n >= ONE_PLANE ? 1 : 2;
     if (!c->batch || !p->m) return DSVC_OK;
     long long at = 0;
     auto take = [&](long long bytes) { const long long o = at; at += (bytes + 1023) / 1024 * 1024; return o; };
