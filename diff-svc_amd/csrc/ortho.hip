@@ -890,11 +890,16 @@ int check_coefficients(const float* c, int steps, double* growth) {
     for (int k = 0; k < 3; ++k)
         if (!isfinite(c[k])) return fail(DSVC_EINVAL, "orthogonalize: coefficient %d is not finite", k);
     for (int k = 0; k < steps; ++k) {
-        double next = 0.0;
-        for (int i = 0; i <= 4096; ++i) {
-            const double s = s_max * i / 4096, l = s * s, f = c[0] + l * (c[1] + l * c[2]);
-            if (fabs(f) > most) most = fabs(f);
-            if (fabs(f * s) > next) next = fabs(f * s);
+        // extrema on [0, s_max], with l = s^2: of f = a + b l + c l^2 at the ends and where b + 2 c l = 0, of s f at the end and where a + 3 b l + 5 c l^2 = 0
+        const double A = c[0], B = c[1], C = c[2], top = s_max * s_max, disc = 9.0 * B * B - 20.0 * A * C;
+        double next = 0.0, at[5] = {0.0, top, C != 0.0 ? -B / (2.0 * C) : -1.0, -1.0, -1.0};
+        if (C != 0.0 && disc >= 0.0) { at[3] = (-3.0 * B + sqrt(disc)) / (10.0 * C); at[4] = (-3.0 * B - sqrt(disc)) / (10.0 * C); }
+        else if (C == 0.0 && B != 0.0) at[3] = -A / (3.0 * B);
+        for (double l : at) {
+            if (!(l >= 0.0 && l <= top)) continue;
+            const double f = fabs(A + l * (B + l * C));
+            if (f > most) most = f;
+            if (f * sqrt(l) > next) next = f * sqrt(l);
         }
         s_max = 1.01 * next;
         if (s_max * s_max > 48.0 || most > 48.0 || s_max > 12.0)

@@ -15,7 +15,7 @@ import torch
 
 from . import _lib
 from ._lib import check, lib
-from .tokens import DTYPES, on_device
+from .tokens import DTYPES, launch
 
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 PLANES = {None: 0, "f16": 1, "f16_x3": 2}
@@ -88,10 +88,7 @@ def orthogonalize(x, steps=5, coefficients=COEFFICIENTS, eps=1e-7, scale=1.0, pr
     cfg = _cfg(v, steps, coefficients, eps, scale, precision)
     L = lib()
     ws, size = _workspace(L, cfg, v)
-    here, stream = on_device(v)
-    with here:
-        rc = L.dsvc_orthogonalize(ctypes.byref(cfg), v.data_ptr(), v.stride(1), v.stride(0), o.data_ptr(), o.stride(1), o.stride(0), ws.data_ptr(), size, stream)
-    check(rc)
+    launch(v, L.dsvc_orthogonalize, ctypes.byref(cfg), v.data_ptr(), v.stride(1), v.stride(0), o.data_ptr(), o.stride(1), o.stride(0), ws.data_ptr(), size)
     return out
 
 
@@ -121,9 +118,6 @@ def muon_step_(param, grad, momentum_buffer, lr, momentum=0.95, nesterov=True, w
     cfg = _cfg(p, steps, coefficients, eps, scale, precision)
     L = lib()
     ws, size = _workspace(L, cfg, p)
-    here, stream = on_device(p)
-    with here:
-        rc = L.dsvc_muon_step(ctypes.byref(cfg), p.data_ptr(), p.stride(1), p.stride(0), g.data_ptr(), g.stride(1), g.stride(0), m.data_ptr(), m.stride(1),
-                              m.stride(0), lr, momentum, nesterov, weight_decay, dev_scale, num_scale, ws.data_ptr(), size, stream)
-    check(rc)
+    launch(p, L.dsvc_muon_step, ctypes.byref(cfg), p.data_ptr(), p.stride(1), p.stride(0), g.data_ptr(), g.stride(1), g.stride(0), m.data_ptr(), m.stride(1),
+           m.stride(0), lr, momentum, nesterov, weight_decay, dev_scale, num_scale, ws.data_ptr(), size)
     return param

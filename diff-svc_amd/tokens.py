@@ -19,30 +19,25 @@ from ._lib import check, lib
 DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 
-def on_device(t):
-    """(context that makes t's device the current one, the raw handle of that device's current stream)."""
+def launch(t, fn, *args):
+    """fn(*args, stream) on t's device and that device's current stream; raises what the library reports."""
     i = t.device.index
-    return torch.cuda.device(i) if i != torch.cuda.current_device() else _here, torch._C._cuda_getCurrentRawStream(i)
-
-
-class _Here:
-    def __enter__(self):
-        pass
-
-    def __exit__(self, *exc):
-        return False
-
-
-_here = _Here()
+    if i == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+    else:
+        with torch.cuda.device(i):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+    if rc:
+        check(rc)
 
 
 def rows_of(t):
     """t with unit stride along its rows and rows that do not overlap (a copy where they do), for a 2-d tensor."""
-    return t if (t.shape[1] <= 1 or t.stride(1) == 1) and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1]) else t.contiguous()
+    return t if t.is_contiguous() or (t.shape[1] <= 1 or t.stride(1) == 1) and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1]) else t.contiguous()
 
 
 def _check_tokens(tokens, other):
-    if tokens.dtype not in (torch.int64, torch.int32):
+    if tokens.dtype is not torch.int64 and tokens.dtype is not torch.int32:
         raise TypeError("diffsvc_amd: tokens must be int32 or int64, got %s" % tokens.dtype)
     if not other.is_cuda or tokens.device != other.device:
         raise RuntimeError("diffsvc_amd: tokens (%s) and tensors (%s) must live on one HIP device; there is no CPU path" % (tokens.device, other.device))
@@ -57,20 +52,18 @@ def _padding(padding_idx, vocab):
 
 
 def _lookup(tokens, weight, scale, flag):
-    if weight.dim() != 2 or not weight.shape[0] or not weight.shape[1]:
-        raise ValueError("the table must be [rows, columns], got %s" % (tuple(weight.shape),))
+    shape = weight.shape
+    if len(shape) != 2 or not shape[0] or not shape[1]:
+        raise ValueError("the table must be [rows, columns], got %s" % (tuple(shape),))
+    V, H = shape
     dtype = DTYPES.get(weight.dtype)
     if dtype is None:
         raise TypeError("diffsvc_amd: tables are float32, float16 or bfloat16, got %s" % weight.dtype)
     _check_tokens(tokens, weight)
-    V, H = weight.shape
     w, t = rows_of(weight), tokens if tokens.is_contiguous() else tokens.contiguous()
-    out = w.new_empty((*tokens.shape, H))
-    here, stream = on_device(w)
-    with here:
-        rc = lib().dsvc_embed_tokens(t.data_ptr(), t.dtype is torch.int64, t.numel(), w.data_ptr(), w.stride(0), V, H, dtype, scale, out.data_ptr(), H,
-                                     None if flag is None else flag.data_ptr(), stream)
-    check(rc)
+    out = w.new_empty((*t.shape, H))
+    launch(w, lib().dsvc_embed_tokens, t.data_ptr(), t.dtype is torch.int64, t.numel(), w.data_ptr(), w.stride(0), V, H, dtype, scale, out.data_ptr(), H,
+           None if flag is None else flag.data_ptr())
     return out
 
 
@@ -100,11 +93,8 @@ def embed_tokens_grad(tokens, dy, vocab, scale=1.0, padding_idx=None, out=None, 
     need = ctypes.c_int64(0)
     check(L.dsvc_embed_tokens_grad_workspace(n, vocab, H, ctypes.byref(need)))
     ws = torch.empty(need.value, device=d.device, dtype=torch.uint8)
-    here, stream = on_device(d)
-    with here:
-        rc = L.dsvc_embed_tokens_grad(t.data_ptr(), t.dtype is torch.int64, n, d.data_ptr(), d.stride(0), DTYPES[d.dtype], vocab, H, scale, pad,
-                                      out.data_ptr(), out.stride(0), DTYPES[out.dtype], accumulate, ws.data_ptr(), need.value, stream)
-    check(rc)
+    launch(d, L.dsvc_embed_tokens_grad, t.data_ptr(), t.dtype is torch.int64, n, d.data_ptr(), d.stride(0), DTYPES[d.dtype], vocab, H, scale, pad, out.data_ptr(),
+           out.stride(0), DTYPES[out.dtype], accumulate, ws.data_ptr(), need.value)
     return out
 
 
@@ -130,7 +120,7 @@ def embed_tokens(tokens, weight, scale=1.0, padding_idx=None, flag=None):
         padding_idx = _padding(padding_idx, weight.shape[0])
     if flag is not None and (flag.dtype != torch.int32 or flag.device != weight.device or flag.numel() < 1):
         raise ValueError("flag must be an int32 tensor on %s" % weight.device)
-    if weight.requires_grad and torch.is_grad_enabled():
+    if weight.requires_grad and torch.is_grad_enabled():           # (a table that takes no gradient has no use for the graph)
         return _EmbedTokens.apply(tokens, weight, scale, padding_idx, flag)
     return _lookup(tokens, weight, scale, flag)
 
