@@ -267,7 +267,8 @@ __global__ __launch_bounds__(256) void k_sort_scatter(SortSrc s, long long n, in
 // ---- 2. chunks of sorted places --------------------------------------------------------------------------------------------------------------
 // Bound by memory: 32768 places of 2048 bf16 columns and a table of 50000 rows take 73 us (339 MB, 4.7 TB/s: a large copy's rate).  Eight rows are in
 // flight per wave, since a gathered row's latency is all there is to hide.  8192 fp32 rows of 256 columns onto 256 rows: 6 us.
-constexpr int ZERO_ROWS = 16;                // rows of dW that one wave looks up and zeroes
+constexpr int ZERO_ROWS = 16, ZERO_SLICES = 4;   // rows of dW that one wave looks up and zeroes, and slices of them (a wave for whole rows: 45 rows of 4245
+                                             // columns take 25 us, when two places are all there is to add)
 
 struct SegArgs {
     const unsigned* keys; const int* order;
@@ -337,7 +338,9 @@ __global__ __launch_bounds__(256) void k_seg_sum(const SegArgs a) {
     const int lane = threadIdx.x & 63;
     const long long unit = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n_seg = a.n_chunks * a.slices;
     if (unit >= n_seg) {                     // zero the rows that no place belongs to
-        const long long v0 = (unit - n_seg) * ZERO_ROWS;
+        const int groups = (a.slices + ZERO_SLICES - 1) / ZERO_SLICES;
+        const long long z = (unit - n_seg) / groups, v0 = z * ZERO_ROWS;
+        const int s0 = (int)(unit - n_seg - z * groups) * ZERO_SLICES, s1 = s0 + ZERO_SLICES < a.slices ? s0 + ZERO_SLICES : a.slices;
         if (a.accumulate || v0 >= a.V) return;
         bool absent = false;
         if (lane < ZERO_ROWS && v0 + lane < a.V) {
@@ -357,7 +360,7 @@ __global__ __launch_bounds__(256) void k_seg_sum(const SegArgs a) {
             const int r = __ffsll((long long)todo) - 1;
             todo &= todo - 1;
             O* p = (O*)a.dw + (v0 + r) * a.dw_ld;
-            for (int s = 0; s < a.slices; ++s) store_row<O, VEC, VECTOR>(p, s * 64 * VEC + (VECTOR ? lane * VEC : lane), a.H, zero);
+            for (int s = s0; s < s1; ++s) store_row<O, VEC, VECTOR>(p, s * 64 * VEC + (VECTOR ? lane * VEC : lane), a.H, zero);
         }
         return;
     }
@@ -527,7 +530,7 @@ int sort_many(const void* tokens, int i64, long long n, long long V, long long p
 template <int TD, int TO, int VEC, bool VECTOR>
 int segments(SegArgs a, hipStream_t st) {
     a.slices = ceil_div(a.H, 64 * VEC);
-    const long long zero = a.accumulate ? 0 : ((long long)a.V + ZERO_ROWS - 1) / ZERO_ROWS, units = a.n_chunks * a.slices + zero;
+    const long long zero = a.accumulate ? 0 : (((long long)a.V + ZERO_ROWS - 1) / ZERO_ROWS) * ceil_div(a.slices, ZERO_SLICES), units = a.n_chunks * a.slices + zero;
     if (units >= (1LL << 26)) return fail(DSVC_EINVAL, "embed_tokens_grad: %lld work items", units);
     if (units) hipLaunchKernelGGL((k_seg_sum<TD, TO, VEC, VECTOR>), dim3((unsigned)((units + 3) / 4)), dim3(256), 0, st, a);
     if (a.n_chunks > 1) hipLaunchKernelGGL((k_seg_join<TO, VEC, VECTOR>), dim3((unsigned)(a.n_chunks - 1), a.slices), dim3(JOIN_WAVES * 64), 0, st, a);
