@@ -112,10 +112,10 @@ __device__ __forceinline__ int block_scan(int v, int* tot) {
     return before + inc - v;
 }
 
-// Up to 16384 tokens in one workgroup and one launch: items stay in registers, each pass exchanges them through LDS.  Digits of up to 10 bits: a table of
+// Up to 8192 tokens in one workgroup and one launch: items stay in registers, each pass exchanges them through LDS.  Digits of up to 10 bits: a table of
 // 256 rows and its ignored places (257 keys) is one pass.  Bound by one CU's latencies (8192 places of 257 keys: 17 us in two passes of 8 bits with the
 // digits scanned in 16 barriers, 11 us in one pass with shuffles).
-constexpr int ONE_MAX = 16384, ONE_BITS = 10;
+constexpr int ONE_MAX = 8192, ONE_BITS = 10;
 template <int IPT>
 __global__ __launch_bounds__(1024) void k_sort_one(const void* __restrict__ tokens, int i64, int n, long long V, long long pad, int passes, int bits, unsigned* __restrict__ keys,
                                                    int* __restrict__ order) {
@@ -140,7 +140,7 @@ __global__ __launch_bounds__(1024) void k_sort_one(const void* __restrict__ toke
 #pragma unroll
         for (int i = 0; i < IPT; ++i) rank[i] = wave_rank((key[i] >> shift) & (bins - 1), bits, lane, (volatile unsigned short*)(cnt + wave * bins));
         __syncthreads();
-        // counts -> first slot of every (wave, digit): over the waves, then over the digits.  (At most 16384 items: slots fit 16 bits.)
+        // counts -> first slot of every (wave, digit): over the waves, then over the digits.  (At most 8192 items: slots fit 16 bits.)
         int run = 0, c[16];
         if ((int)threadIdx.x < bins) {
 #pragma unroll
@@ -477,16 +477,18 @@ int grad_plan(int64_t n, int64_t V, int32_t H, int esize, GradPlan* p) {
     *p = GradPlan{};
     int bits = 1;
     while ((V >> bits) != 0) ++bits;         // keys 0 ... V
-    // one workgroup: 8192 places in one pass 11 us, 16384 in two 47 us, where two passes of two launches take 25 us
-    p->one = bits <= ONE_BITS ? n <= ONE_MAX : n <= ONE_MAX / 4;
+    // one workgroup or two launches a pass, the whole operator on 64 columns: 8192 places of 1000 rows 22 / 29 us, 16384 38 / 31; two passes: 4096 of 5000
+    // rows 19 / 28
+    p->one = bits <= ONE_BITS ? n <= ONE_MAX : n <= ONE_MAX / 2;
     const int most = p->one ? ONE_BITS : 8;
     p->passes = (bits + most - 1) / most;
     p->bits = (bits + p->passes - 1) / p->passes;
-    p->ipt = p->one ? (n <= 1024 ? 1 : n <= 2048 ? 2 : n <= 4096 ? 4 : n <= 8192 ? 8 : 16) : (n <= FEW_BLOCKS * 1024 ? 4 : n <= FEW_BLOCKS * 2048 ? 8 : 16);
-    // chunks: enough waves to fill the chip (16 a CU) from few tokens, few partial rows in a run from many
+    p->ipt = p->one ? (n <= 1024 ? 1 : n <= 2048 ? 2 : n <= 4096 ? 4 : 8) : (n <= FEW_BLOCKS * 1024 ? 4 : n <= FEW_BLOCKS * 2048 ? 8 : 16);
+    // chunks: 16 waves a CU (32768 places of 50000 rows, 2048 bf16 columns 108 us, 8 a CU: 113; a single token's partial rows would have fewer: 100000 of 256
+    // fp32 columns 103 us, 80); at least 8 places, 16 from 4096 slices on (8192 places of one token, 256 columns: 30 -> 25 us; 500 places of 64: 10 -> 12)
     const long long slices = (H + 64 * (16 / esize) - 1) / (64 * (16 / esize));
     const long long want = n * slices / 4096;
-    p->chunk = (int)(want < 8 ? 8 : want > 2048 ? 2048 : (want + 7) / 8 * 8);
+    p->chunk = (int)(want < 1 ? 8 : want < 16 ? 16 : want > 2048 ? 2048 : (want + 7) / 8 * 8);
     p->n_chunks = (n + p->chunk - 1) / p->chunk;
     p->blocks = (n + 256 * p->ipt - 1) / (256 * p->ipt);
     long long at = 0;
@@ -601,8 +603,7 @@ int dsvc_embed_tokens_grad(const void* tokens, int32_t tokens_i64, int64_t n, co
         if (p.ipt == 1) DSVC_TRY(sort_one<1>(tokens, i64, m, vocab, padding_idx, p, keys[0], order[0], st));
         else if (p.ipt == 2) DSVC_TRY(sort_one<2>(tokens, i64, m, vocab, padding_idx, p, keys[0], order[0], st));
         else if (p.ipt == 4) DSVC_TRY(sort_one<4>(tokens, i64, m, vocab, padding_idx, p, keys[0], order[0], st));
-        else if (p.ipt == 8) DSVC_TRY(sort_one<8>(tokens, i64, m, vocab, padding_idx, p, keys[0], order[0], st));
-        else DSVC_TRY(sort_one<16>(tokens, i64, m, vocab, padding_idx, p, keys[0], order[0], st));
+        else DSVC_TRY(sort_one<8>(tokens, i64, m, vocab, padding_idx, p, keys[0], order[0], st));
     } else if (n > 0) {
         int* hist = (int*)(ws + p.off_hist);
         if (p.ipt == 4) DSVC_TRY(sort_many<4>(tokens, i64, n, vocab, padding_idx, p, hist, keys, order, &at, st));
