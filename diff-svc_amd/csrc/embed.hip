@@ -14,6 +14,8 @@
 // A token that fills the batch costs what a batch of different tokens costs.
 #include <math.h>
 
+#include <type_traits>
+
 #include "../../include/dsvc.h"
 #include "common.h"
 
@@ -173,8 +175,8 @@ __global__ __launch_bounds__(1024) void k_sort_one(const void* __restrict__ toke
         }
 }
 
-// More tokens: blocks of 256 IPT, up to 8 bits a pass, counts as hist[digit][block].  The first pass reads the tokens themselves (keys == nullptr).
-// Up to 64 blocks a block finds its first slots from the whole table of counts itself (64 KiB in L2): two launches a pass.  Beyond, the table is
+// More tokens: blocks of 256 IPT, up to 8 bits a pass or 9 (D = 1 or 2 digits to a thread), counts as hist[digit][block].  The first pass reads the tokens
+// themselves (keys == nullptr).  Up to 64 blocks a block finds its first slots from the whole table of counts itself (64 D KiB in L2): two launches a pass.  Beyond, the table is
 // scanned by a launch of its own.  (Counting a pass's digits while the pass before it scatters saves a launch, but its atomics meet at a skewed
 // text's few digits: 32768 places 31 us instead of 7.5 + 4.7.)
 constexpr int FEW_BLOCKS = 64;
@@ -184,10 +186,11 @@ __device__ __forceinline__ void sort_load(const SortSrc& s, long long i, long lo
     key = s.keys ? s.keys[i] : key_of(token_at(s.tokens, s.i64, i), s.V, s.pad);
     idx = s.keys ? s.order[i] : (int)i;
 }
-template <int IPT>
+template <int IPT, int D>
 __global__ __launch_bounds__(256) void k_sort_hist(SortSrc s, long long n, int shift, int mask, int* __restrict__ hist, int ld) {
-    __shared__ int cnt[256];
-    cnt[threadIdx.x] = 0;
+    __shared__ int cnt[256 * D];
+#pragma unroll
+    for (int d = 0; d < D; ++d) cnt[256 * d + threadIdx.x] = 0;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < IPT; ++i) {
@@ -197,7 +200,8 @@ __global__ __launch_bounds__(256) void k_sort_hist(SortSrc s, long long n, int s
         if (at < n) atomicAdd(&cnt[(key >> shift) & mask], 1);
     }
     __syncthreads();
-    hist[(long long)threadIdx.x * ld + blockIdx.x] = cnt[threadIdx.x];
+#pragma unroll
+    for (int d = 0; d < D; ++d) hist[(long long)(256 * d + threadIdx.x) * ld + blockIdx.x] = cnt[256 * d + threadIdx.x];
 }
 __global__ __launch_bounds__(1024) void k_sort_scan(int* __restrict__ hist, int n) {      // exclusive scan in place
     __shared__ int tot[16];
@@ -218,42 +222,54 @@ __global__ __launch_bounds__(1024) void k_sort_scan(int* __restrict__ hist, int 
     }
 }
 // FEW: hist holds counts (ld = FEW_BLOCKS); else first slots
-template <int IPT, bool FEW>
+template <int IPT, int D, bool FEW>
 __global__ __launch_bounds__(256) void k_sort_scatter(SortSrc s, long long n, int shift, int bits, const int* __restrict__ hist, int ld, unsigned* __restrict__ keys,
                                                       int* __restrict__ order) {
-    __shared__ int cnt[4][256];
+    __shared__ int cnt[4][256 * D];
     __shared__ int tot[4];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, mask = (1 << bits) - 1;
-    for (int w = 0; w < 4; ++w) cnt[w][threadIdx.x] = 0;
+    for (int i = threadIdx.x; i < 4 * 256 * D; i += 256) cnt[0][i] = 0;
     __syncthreads();
     const long long first = (long long)blockIdx.x * (256 * IPT) + wave * 64 * IPT + lane;
     unsigned key[IPT];
     int idx[IPT], rank[IPT];
 #pragma unroll
     for (int i = 0; i < IPT; ++i) sort_load(s, first + i * 64, n, key[i], idx[i]);
-    int run = 0;
+    int run[D];                              // digits D threadIdx.x + d
     if (FEW) {
-        int all = 0;
-        const int4* h = (const int4*)(hist + threadIdx.x * FEW_BLOCKS);
+        int all[D], sum = 0;
 #pragma unroll
-        for (int q = 0; q < FEW_BLOCKS / 4; ++q) {
-            const int4 v = h[q];
-            const int e[4] = {v.x, v.y, v.z, v.w};
+        for (int d = 0; d < D; ++d) {
+            all[d] = run[d] = 0;
+            const int4* h = (const int4*)(hist + (D * threadIdx.x + d) * FEW_BLOCKS);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int c = 4 * q + k < (int)gridDim.x ? e[k] : 0;
-                all += c;
-                run += 4 * q + k < (int)blockIdx.x ? c : 0;
+            for (int q = 0; q < FEW_BLOCKS / 4; ++q) {
+                const int4 v = h[q];
+                const int e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int c = 4 * q + k < (int)gridDim.x ? e[k] : 0;
+                    all[d] += c;
+                    run[d] += 4 * q + k < (int)blockIdx.x ? c : 0;
+                }
             }
+            sum += all[d];
         }
-        run += block_scan<4>(all, tot);
-    } else run = hist[(long long)threadIdx.x * ld + blockIdx.x];
+        int base = block_scan<4>(sum, tot);
+#pragma unroll
+        for (int d = 0; d < D; ++d) { run[d] += base; base += all[d]; }
+    } else {
+#pragma unroll
+        for (int d = 0; d < D; ++d) run[d] = hist[(long long)(D * threadIdx.x + d) * ld + blockIdx.x];
+    }
 #pragma unroll
     for (int i = 0; i < IPT; ++i) rank[i] = wave_rank((key[i] >> shift) & mask, bits, lane, (volatile int*)cnt[wave]);
     __syncthreads();
     // this block's slots of a digit start at `run`; the waves' shares follow one another.  Items behind the end have the highest digit and come
     // last in the last block: they take no slot of another's
-    for (int w = 0; w < 4; ++w) { const int c = cnt[w][threadIdx.x]; cnt[w][threadIdx.x] = run; run += c; }
+#pragma unroll
+    for (int d = 0; d < D; ++d)
+        for (int w = 0; w < 4; ++w) { const int c = cnt[w][D * threadIdx.x + d]; cnt[w][D * threadIdx.x + d] = run[d]; run[d] += c; }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < IPT; ++i)
@@ -466,7 +482,7 @@ inline int size_of(int dtype) { return dtype == F32 ? 4 : 2; }
 inline bool known(int dtype) { return dtype == F32 || dtype == F16 || dtype == BF16; }
 
 struct GradPlan {
-    int passes, bits, one, ipt, chunk;
+    int passes, bits, one, ipt, digits, chunk;    // digits: 256 of them, or 512
     long long n_chunks, blocks, off_k[2], off_o[2], off_hist, off_part, bytes;
 };
 
@@ -480,9 +496,11 @@ int grad_plan(int64_t n, int64_t V, int32_t H, int esize, GradPlan* p) {
     // one workgroup or two launches a pass, the whole operator on 64 columns: 8192 places of 1000 rows 22 / 29 us, 16384 38 / 31; two passes: 4096 of 5000
     // rows 19 / 28
     p->one = bits <= ONE_BITS ? n <= ONE_MAX : n <= ONE_MAX / 2;
-    const int most = p->one ? ONE_BITS : 8;
+    // digits of 9 bits where they save a pass (114310 places of 83939 rows, 30 columns: 73 -> 67 us, 9000 of 300 rows 28 -> 22)
+    const int most = p->one ? ONE_BITS : (bits + 8) / 9 < (bits + 7) / 8 ? 9 : 8;
     p->passes = (bits + most - 1) / most;
     p->bits = (bits + p->passes - 1) / p->passes;
+    p->digits = p->bits > 8 ? 512 : 256;
     p->ipt = p->one ? (n <= 1024 ? 1 : n <= 2048 ? 2 : n <= 4096 ? 4 : 8) : (n <= FEW_BLOCKS * 1024 ? 4 : n <= FEW_BLOCKS * 2048 ? 8 : 16);
     // chunks: 16 waves a CU (32768 places of 50000 rows, 2048 bf16 columns 108 us, 8 a CU: 113; a single token's partial rows would have fewer: 100000 of 256
     // fp32 columns 103 us, 80); at least 8 places, 16 from 4096 slices on (8192 places of one token, 256 columns: 30 -> 25 us; 500 places of 64: 10 -> 12)
@@ -494,7 +512,7 @@ int grad_plan(int64_t n, int64_t V, int32_t H, int esize, GradPlan* p) {
     long long at = 0;
     auto take = [&](long long bytes) { const long long o = at; at += (bytes + 255) / 256 * 256; return o; };
     for (int i = 0; i < (p->one ? 1 : 2); ++i) { p->off_k[i] = take(n * 4); p->off_o[i] = take(n * 4); }
-    if (!p->one) p->off_hist = take(256 * (p->blocks <= FEW_BLOCKS ? FEW_BLOCKS : p->blocks) * 4);
+    if (!p->one) p->off_hist = take(p->digits * (p->blocks <= FEW_BLOCKS ? FEW_BLOCKS : p->blocks) * 4);
     p->off_part = take(p->n_chunks * 2 * H * 4);
     p->bytes = at < 256 ? 256 : at;
     return DSVC_OK;
@@ -509,7 +527,7 @@ int sort_one(const void* tokens, int i64, int n, long long V, long long pad, con
     return DSVC_OK;
 }
 // returns through `at` which of the two buffers holds the result
-template <int IPT>
+template <int IPT, int D>
 int sort_many(const void* tokens, int i64, long long n, long long V, long long pad, const GradPlan& p, int* hist, unsigned* const (&keys)[2], int* const (&order)[2], int* at,
               hipStream_t st) {
     const dim3 grid((unsigned)p.blocks), block(256);
@@ -518,11 +536,11 @@ int sort_many(const void* tokens, int i64, long long n, long long V, long long p
     for (int k = 0; k < p.passes; ++k) {
         const SortSrc s{tokens, i64, V, pad, k ? keys[(k + 1) & 1] : nullptr, k ? order[(k + 1) & 1] : nullptr};
         *at = k & 1;
-        hipLaunchKernelGGL(k_sort_hist<IPT>, grid, block, 0, st, s, n, p.bits * k, mask, hist, ld);
-        if (few) hipLaunchKernelGGL((k_sort_scatter<IPT, true>), grid, block, 0, st, s, n, p.bits * k, p.bits, hist, ld, keys[*at], order[*at]);
+        hipLaunchKernelGGL((k_sort_hist<IPT, D>), grid, block, 0, st, s, n, p.bits * k, mask, hist, ld);
+        if (few) hipLaunchKernelGGL((k_sort_scatter<IPT, D, true>), grid, block, 0, st, s, n, p.bits * k, p.bits, hist, ld, keys[*at], order[*at]);
         else {
-            hipLaunchKernelGGL(k_sort_scan, dim3(1), dim3(1024), 0, st, hist, (int)(256 * p.blocks));
-            hipLaunchKernelGGL((k_sort_scatter<IPT, false>), grid, block, 0, st, s, n, p.bits * k, p.bits, hist, ld, keys[*at], order[*at]);
+            hipLaunchKernelGGL(k_sort_scan, dim3(1), dim3(1024), 0, st, hist, (int)(256 * D * p.blocks));
+            hipLaunchKernelGGL((k_sort_scatter<IPT, D, false>), grid, block, 0, st, s, n, p.bits * k, p.bits, hist, ld, keys[*at], order[*at]);
         }
     }
     DSVC_HIP(hipGetLastError());
@@ -606,9 +624,13 @@ int dsvc_embed_tokens_grad(const void* tokens, int32_t tokens_i64, int64_t n, co
         else DSVC_TRY(sort_one<8>(tokens, i64, m, vocab, padding_idx, p, keys[0], order[0], st));
     } else if (n > 0) {
         int* hist = (int*)(ws + p.off_hist);
-        if (p.ipt == 4) DSVC_TRY(sort_many<4>(tokens, i64, n, vocab, padding_idx, p, hist, keys, order, &at, st));
-        else if (p.ipt == 8) DSVC_TRY(sort_many<8>(tokens, i64, n, vocab, padding_idx, p, hist, keys, order, &at, st));
-        else DSVC_TRY(sort_many<16>(tokens, i64, n, vocab, padding_idx, p, hist, keys, order, &at, st));
+        auto sort = [&](auto digits) {
+            constexpr int D = decltype(digits)::value;
+            if (p.ipt == 4) return sort_many<4, D>(tokens, i64, n, vocab, padding_idx, p, hist, keys, order, &at, st);
+            if (p.ipt == 8) return sort_many<8, D>(tokens, i64, n, vocab, padding_idx, p, hist, keys, order, &at, st);
+            return sort_many<16, D>(tokens, i64, n, vocab, padding_idx, p, hist, keys, order, &at, st);
+        };
+        DSVC_TRY(p.digits == 512 ? sort(std::integral_constant<int, 2>{}) : sort(std::integral_constant<int, 1>{}));
     }
     const SegArgs a{keys[at], order[at], n, (unsigned)vocab, H, p.chunk, 0, p.n_chunks, dy, dy_ld, dw, dw_ld, (float*)(ws + p.off_part), scale, accumulate != 0};
     const int ds = size_of(dy_dtype), os = size_of(dw_dtype);

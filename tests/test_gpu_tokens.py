@@ -98,6 +98,18 @@ def test_gradient(dtype, kind, N, V, H):
     assert torch.equal(got, T.embed_tokens_grad(t.cuda(), dy.cuda(), V, scale=scale, padding_idx=pad))       # fixed order of sums
 
 
+@pytest.mark.parametrize("kind", ["zipf", "one", "even"])
+@pytest.mark.parametrize("N, V, H", [
+    (9000, 300, 5), (9000, 255, 5), (5000, 70000, 6), (70000, 510, 3), (140000, 70000, 2), (270000, 200, 1), (270000, 300, 2), (300000, 131071, 2)])
+def test_gradient_of_long_texts(kind, N, V, H):
+    """Sorts of several blocks: digits of 8 and 9 bits, 4 to 16 places a thread, up to 64 blocks and more."""
+    g = torch.Generator().manual_seed(N + V)
+    t, dy = ids(kind, N, V, g), torch.randn(N, H, generator=g) * 0.1
+    got = T.embed_tokens_grad(t.cuda(), dy.cuda(), V, scale=0.5, padding_idx=1)
+    check_grad(got, *grad64(t, dy, V, 0.5, 1))
+    assert torch.equal(got, T.embed_tokens_grad(t.int().cuda(), dy.cuda(), V, scale=0.5, padding_idx=1))
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_gradient_outputs(dtype):
     """float32 results of any type, accumulation, strided gradients and outputs, broadcast gradients, tokens outside the table, no tokens."""
