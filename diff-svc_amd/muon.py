@@ -58,7 +58,7 @@ def _matrices(name, t, copy):
     """t as [batch, rows, columns] with unit stride along the rows; ``copy``: in a new tensor where it does not lie so, else refused."""
     m, n = t.shape[-2:]
     d = t.dim()
-    v = t if d == 3 else t.unsqueeze(0) if d == 2 else t.reshape(-1, m, n) if copy else t.view(-1, m, n)
+    v = t if d == 3 else t.unsqueeze(0) if d == 2 else t.reshape(math.prod(t.shape[:-2]), m, n) if copy else t.view(math.prod(t.shape[:-2]), m, n)
     bs, ld, one = v.stride()
     if (n <= 1 or one == 1) and (m <= 1 or ld >= n) and (v.shape[0] <= 1 or bs >= (m - 1) * ld + n):
         return v

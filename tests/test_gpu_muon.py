@@ -221,6 +221,14 @@ def test_muon_step_refusals():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(0, 3, 4), (2, 0, 3, 4), (2, 2, 0, 5), (2, 3, 4, 0)])
+def test_nothing_to_do(shape):
+    x = torch.zeros(shape, device="cuda")
+    assert M.orthogonalize(x).shape == shape
+    assert M.muon_step_(x, torch.zeros_like(x), torch.zeros_like(x), 0.1).shape == shape
+
+
+@pytest.mark.gpu
 def test_streams_and_graph_replay():
     g = update((2, 200, 300), 8).cuda()
     want = M.orthogonalize(g)
