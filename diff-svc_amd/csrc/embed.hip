@@ -431,7 +431,7 @@ __global__ __launch_bounds__(256) void k_seg_sum(const SegArgs a) {
 }
 
 // ---- 3. runs that span chunks: grid (chunks, slices), eight waves.  Most blocks find nothing to close, most runs a few chunks: latency counts, so the
-// lanes of a wave look at the first places of 64 chunks at once and only longer runs are searched (8192 places 4.2 us, 32768 of 2048 columns 11 us; 16 waves
+// lanes of a wave look at the first places of 64 chunks at once and only longer runs are searched (8192 places 3.6 us, 32768 of 2048 columns 11 us; 16 waves
 // spill) ----
 constexpr int JOIN_WAVES = 8;
 template <int TO, int VEC, bool VECTOR>
@@ -503,10 +503,10 @@ int grad_plan(int64_t n, int64_t V, int32_t H, int esize, GradPlan* p) {
     p->digits = p->bits > 8 ? 512 : 256;
     p->ipt = p->one ? (n <= 1024 ? 1 : n <= 2048 ? 2 : n <= 4096 ? 4 : 8) : (n <= FEW_BLOCKS * 1024 ? 4 : n <= FEW_BLOCKS * 2048 ? 8 : 16);
     // chunks: 16 waves a CU (32768 places of 50000 rows, 2048 bf16 columns 108 us, 8 a CU: 113; a single token's partial rows would have fewer: 100000 of 256
-    // fp32 columns 103 us, 80); at least 8 places, 16 from 4096 slices on (8192 places of one token, 256 columns: 30 -> 25 us; 500 places of 64: 10 -> 12)
+    // fp32 columns 103 us, 80); at least 8 places, 16 from 8192 slices on (8192 places of one token, 256 columns: 30 -> 25 us; 500 places of 64: 10 -> 12)
     const long long slices = (H + 64 * (16 / esize) - 1) / (64 * (16 / esize));
     const long long want = n * slices / 4096;
-    p->chunk = (int)(want < 1 ? 8 : want < 16 ? 16 : want > 2048 ? 2048 : (want + 7) / 8 * 8);
+    p->chunk = (int)(want < 2 ? 8 : want < 16 ? 16 : want > 2048 ? 2048 : (want + 7) / 8 * 8);
     p->n_chunks = (n + p->chunk - 1) / p->chunk;
     p->blocks = (n + 256 * p->ipt - 1) / (256 * p->ipt);
     long long at = 0;

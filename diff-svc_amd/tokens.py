@@ -69,7 +69,7 @@ def _lookup(tokens, weight, scale, flag):
 
 def embed_tokens_grad(tokens, dy, vocab, scale=1.0, padding_idx=None, out=None, accumulate=False):
     """Gradient of ``embed_tokens`` in its table, [vocab, H]: dy is [..., H] over tokens of shape [...].  ``out`` (dy's type or float32) is
-    written whole, zeros where a token does not occur; with ``accumulate`` the sums are added to what it holds instead."""
+    written whole, zeros where a token does not occur; with ``accumulate`` the sums are added to what it holds instead.  It does not overlap dy."""
     if dy.dtype not in DTYPES:
         raise TypeError("diffsvc_amd: gradients are float32, float16 or bfloat16, got %s" % dy.dtype)
     if dy.dim() < 1 or tuple(dy.shape[:-1]) != tuple(tokens.shape) or not dy.shape[-1]:
