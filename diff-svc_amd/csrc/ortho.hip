@@ -5,10 +5,11 @@
 //   steps times:  A = X X^T,  M = a I + b A + c A A,  X <- M X            (the singular values go through s (a + b s^2 + c s^4))
 //   O = scale * X                (transposed back)
 //
-// Arithmetic: every product is an fp16 MFMA (v_mfma_f32_32x32x16_f16) with fp32 accumulation.  Large bf16 tensors run on ONE fp16 plane (its 11 bits stay
-// below the 8 of the result: 1.2e-3 against a half step of 1.7e-3 rms); the rest on hi + lo planes and three MFMAs per product (hi hi + hi lo +
-// lo hi: 22 bits per operand, fp32-class, the trainer's own scheme).  Small bf16 tensors too: launches bound them, not products, and the
-// roundings of few elements do not average (2.9e-3 on one plane at [8, 24]).
+// Arithmetic: every product is an fp16 MFMA (v_mfma_f32_32x32x16_f16) with fp32 accumulation, on hi + lo planes and three MFMAs per product (hi hi + hi lo +
+// lo hi: 22 bits per operand, fp32-class, the trainer's own scheme), whatever the tensor's type: a rounding of an early iterate grows by up to a^steps
+// (485 for the usual five) in the directions in which the update has next to nothing.  [512, 768] of rank 1: 1.1e-4 of the result's norm from exact (fp32
+// products 6e-5), of full rank 2.5e-6.  ONE plane is the caller's own choice (cfg.planes = 1): a third of the MFMAs, 11 bits, and so 1.9e-3 at full
+// rank but 4e-2 at rank 16 and 1e-1 at rank 1, where a bf16 result's own rounding is 1.7e-3.
 // The planes hold X * 2^12 and A, M * 2^10: |X| and |M| are bounded by the polynomial on [0, 1] (checked on the host for the caller's
 // coefficients), so fp16's top is out of reach and small elements keep their bits; an update whose norm eps swamps is carried with an
 // extra power of two that shrinks as the iterate grows (Scalars::e0).  Norms are summed in fp64: no square of a tiny gradient underflows.
@@ -42,7 +43,6 @@ constexpr int PAD = 128;                     // rows and columns of every interm
 // Padded elements up to which one workgroup takes a matrix of up to 64 rows.  fp32, one workgroup against 17 launches (GPU time; the host takes 60 us to
 // launch them): [1, 1] 24 / 71 us, [64, 64] x 8 27 / 76, [64, 256] 52 / 80, [32, 500] 72 / 88, [64, 1024] 163 / 103; [48, 64] x 2000 197 / 1162
 constexpr long long ONE_WORK = 16384;
-constexpr double ONE_PLANE = 1 << 27;        // multiply-adds of a product of the batch from which bf16 takes one plane
 constexpr int ONE_LDS = 156 * 1024;          // its LDS (the rest: static)
 constexpr int SUM_BLOCKS = 256;              // partial sums of squares per matrix
 
@@ -883,7 +883,7 @@ int check_coefficients(const float* c, int steps, double* growth) {
 int make_plan(const dsvc_ortho_cfg* c, Plan* p) {
     if (!c) return fail(DSVC_EINVAL, "null argument");
     if (c->dtype < F32 || c->dtype > BF16) return fail(DSVC_EINVAL, "orthogonalize: unknown type %d", c->dtype);
-    if (c->planes != 0 && c->planes != 1 && c->planes != 2) return fail(DSVC_EINVAL, "orthogonalize: %d planes (1, 2 or 0: by type)", c->planes);
+    if (c->planes != 0 && c->planes != 1 && c->planes != 2) return fail(DSVC_EINVAL, "orthogonalize: %d planes (1, 2 or 0: 2)", c->planes);
     if (c->batch < 0 || c->rows < 0 || c->cols < 0) return fail(DSVC_EINVAL, "orthogonalize: bad shape [%d, %d, %d]", c->batch, c->rows, c->cols);
     if (c->rows > (1 << 20) || c->cols > (1 << 20) || c->batch > 65535) return fail(DSVC_EINVAL, "orthogonalize: shape [%d, %d, %d] is too large", c->batch, c->rows, c->cols);
     if (c->steps < 1 || c->steps > 64) return fail(DSVC_EINVAL, "orthogonalize: %d steps", c->steps);
@@ -896,7 +896,7 @@ int make_plan(const dsvc_ortho_cfg* c, Plan* p) {
     p->tall = c->rows > c->cols;
     p->m = p->tall ? c->cols : c->rows;
     p->n = p->tall ? c->rows : c->cols;
-    p->P = c->planes ? c->planes : c->dtype == BF16 && (double)c->batch * p->m * p->m * p->n >= ONE_PLANE ? 1 : 2;
+    p->P = c->planes ? c->planes : 2;
     if (!c->batch || !p->m) return DSVC_OK;
     long long at = 0;
     auto take = [&](long long bytes) { const long long o = at; at += (bytes + 1023) / 1024 * 1024; return o; };

@@ -403,7 +403,7 @@ DSVC_API int dsvc_embed_tokens_grad(const void* tokens, int32_t tokens_i64, int6
 
 typedef struct {
     int32_t dtype;            /* DSVC_DTYPE_* of the tensor(s) */
-    int32_t planes;           /* fp16 planes per operand of the products: 1, 2 (fp32-class) or 0 = 1 for bf16 batches of 2^27 multiply-adds a product, else 2 */
+    int32_t planes;           /* fp16 planes per operand of the products: 2 (fp32-class), 0 = 2, or 1: a third of the work, errors of 2e-3 (full rank) ... 1e-1 (rank 1) */
     int32_t batch, rows, cols;
     int32_t steps;            /* 1 ... 64 */
     float coef[3];            /* a, b, c: one step takes a singular value s to s (a + b s^2 + c s^4) */
