@@ -12,6 +12,7 @@ import ctypes
 
 import torch
 from torch import nn
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import check, lib
@@ -100,10 +101,15 @@ def embed_tokens_grad(tokens, dy, vocab, scale=1.0, padding_idx=None, out=None, 
 
 class _EmbedTokens(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, tokens, weight, scale, padding_idx, flag):
-        ctx.save_for_backward(tokens)
-        ctx.args = weight.shape[0], scale, padding_idx
+    def forward(tokens, weight, scale, padding_idx, flag):
         return _lookup(tokens, weight, scale, flag)
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        tokens, weight, scale, padding_idx, _ = inputs
+        ctx.save_for_backward(tokens)
+        ctx.save_for_forward(tokens)
+        ctx.args = weight.shape[0], scale, padding_idx
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -111,16 +117,21 @@ class _EmbedTokens(torch.autograd.Function):
         vocab, scale, padding_idx = ctx.args
         return None, embed_tokens_grad(ctx.saved_tensors[0], dy, vocab, scale, padding_idx), None, None, None
 
+    @staticmethod
+    def jvp(ctx, _, dw, *__):                      # linear in the table; its row padding_idx counts forwards, as in nn.Embedding
+        return _EmbedTokens.apply(ctx.saved_tensors[0], dw, ctx.args[1], ctx.args[2], None)
+
 
 def embed_tokens(tokens, weight, scale=1.0, padding_idx=None, flag=None):
-    """scale * weight[tokens], [..., H] for tokens [...]; differentiable in ``weight``, whose row ``padding_idx`` gets no gradient.  flag: an int32
-    device tensor that is set to 1 where a token lies outside the table (its row is zero)."""
+    """scale * weight[tokens], [..., H] for tokens [...]; differentiable in ``weight`` (backwards and forwards), whose row ``padding_idx`` gets no gradient.
+    flag: an int32 device tensor that is set to 1 where a token lies outside the table (its row is zero)."""
     scale = float(scale)
     if padding_idx is not None:
         padding_idx = _padding(padding_idx, weight.shape[0])
     if flag is not None and (flag.dtype != torch.int32 or flag.device != weight.device or flag.numel() < 1):
         raise ValueError("flag must be an int32 tensor on %s" % weight.device)
-    if weight.requires_grad and torch.is_grad_enabled():           # (a table that takes no gradient has no use for the graph)
+    # (a table that takes no gradient and has no tangent has no use for the graph)
+    if weight.requires_grad and torch.is_grad_enabled() or forward_ad._current_level >= 0:
         return _EmbedTokens.apply(tokens, weight, scale, padding_idx, flag)
     return _lookup(tokens, weight, scale, flag)
 

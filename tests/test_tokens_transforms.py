@@ -1,0 +1,81 @@
+"""The lookup under torch's transforms, against nn.functional.embedding under the same: forward-mode derivatives.  On the device, and on the
+host with the two kernel launches replaced by numpy -- code that no transform can look into, as the kernels are."""
+import numpy as np
+import pytest
+import torch
+import torch.nn.functional as F
+from torch.autograd import forward_ad as fw
+
+import diffsvc_amd  # noqa: F401
+from diffsvc_amd import tokens as T
+
+V, H, PAD, SCALE = 11, 8, 3, 2.0                       # sums of few small integers: exact in every order
+
+
+def _lookup(tokens, weight, scale, flag):
+    t, w = tokens.numpy(), weight.detach().numpy()
+    ok = (t >= 0) & (t < w.shape[0])
+    if flag is not None and not ok.all():
+        flag.fill_(1)
+    return torch.from_numpy(np.where(ok[..., None], w[np.where(ok, t, 0)] * np.float32(scale), np.float32(0)).astype(np.float32))
+
+
+def _grad(tokens, dy, vocab, scale=1.0, padding_idx=None):
+    t, d = tokens.numpy().reshape(-1), dy.detach().numpy().reshape(tokens.numel(), -1)
+    ok = (t >= 0) & (t < vocab) & (t != (-1 if padding_idx is None else padding_idx))
+    w = np.zeros((vocab, d.shape[1]), np.float32)
+    np.add.at(w, t[ok], d[ok] * np.float32(scale))
+    return torch.from_numpy(w)
+
+
+@pytest.fixture(params=["host", pytest.param("cuda", marks=pytest.mark.gpu)])
+def dev(request, monkeypatch):
+    if request.param == "host":
+        monkeypatch.setattr(T, "_lookup", _lookup)
+        monkeypatch.setattr(T, "embed_tokens_grad", _grad)
+        return "cpu"
+    return "cuda"
+
+
+def small(*shape, seed=0, dev="cpu"):
+    return torch.randint(-4, 5, shape, generator=torch.Generator().manual_seed(seed)).float().to(dev)
+
+
+def tokens(dev, *shape, seed=1):
+    return torch.randint(0, V, shape, generator=torch.Generator().manual_seed(seed)).to(dev)
+
+
+def plain(t, w):
+    return F.embedding(t, w, padding_idx=PAD) * SCALE
+
+
+def ours(t, w, flag=None):
+    return T.embed_tokens(t, w, SCALE, PAD, flag)
+
+
+@pytest.mark.parametrize("grad", [False, True])
+@pytest.mark.parametrize("mode", [True, False])
+def test_forward_mode(dev, grad, mode):
+    """The table's tangent reaches the output: frozen and trained tables, with grad mode on and off."""
+    w, dw, t = small(V, H, dev=dev).requires_grad_(grad), small(V, H, seed=2, dev=dev), tokens(dev, 4, 5)
+    with fw.dual_level(), torch.set_grad_enabled(mode):
+        got, want = (fw.unpack_dual(f(t, fw.make_dual(w, dw))) for f in (ours, plain))
+        assert torch.equal(got.primal, want.primal) and torch.equal(got.tangent, want.tangent) and got.tangent.any()
+        assert fw.unpack_dual(ours(t, w)).tangent is None
+    assert got.primal.requires_grad == (grad and mode)
+    if grad and mode:
+        got.primal.sum().backward()
+        assert not w.grad[PAD].any() and w.grad.any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("trained", [False, True])
+def test_forward_mode_of_the_module(trained):
+    m, e = T.TokenEmbeddingHip(V, H, padding_idx=PAD).cuda(), torch.nn.Embedding(V, H, padding_idx=PAD).cuda()
+    m.load_state_dict(e.state_dict())
+    for x in (m, e):
+        x.requires_grad_(trained)
+    dw, t = small(V, H, seed=2, dev="cuda"), tokens("cuda", 7)
+    with fw.dual_level():
+        a, b = (torch.func.functional_call(x, {"weight": fw.make_dual(x.weight, dw)}, (t,)) for x in (m, e))
+        assert torch.equal(fw.unpack_dual(a).tangent, fw.unpack_dual(b).tangent) and torch.equal(a, b)
