@@ -22,6 +22,8 @@ DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 def launch(t, fn, *args):
     """fn(*args, stream) on t's device and that device's current stream; raises what the library reports."""
+    if torch._C._get_tracing_state() is not None:
+        raise RuntimeError("diffsvc_amd: a trace would record the memory of this call without the kernels that fill it")
     i = t.device.index
     if i == torch._C._cuda_getDevice():
         rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
@@ -126,6 +128,8 @@ def embed_tokens(tokens, weight, scale=1.0, padding_idx=None, flag=None):
     """scale * weight[tokens], [..., H] for tokens [...]; differentiable in ``weight`` (backwards and forwards), whose row ``padding_idx`` gets no gradient.
     flag: an int32 device tensor that is set to 1 where a token lies outside the table (its row is zero)."""
     scale = float(scale)
+    if torch._C._get_tracing_state() is not None:                  # a trace sees no kernel launch: it records the operator
+        return torch.ops.diffsvc_amd.embed_tokens(tokens, weight, scale, padding_idx, flag)
     if padding_idx is not None:
         padding_idx = _padding(padding_idx, weight.shape[0])
     if flag is not None and (flag.dtype != torch.int32 or flag.device != weight.device or flag.numel() < 1):
@@ -134,6 +138,12 @@ def embed_tokens(tokens, weight, scale=1.0, padding_idx=None, flag=None):
     if weight.requires_grad and torch.is_grad_enabled() or forward_ad._current_level >= 0:
         return _EmbedTokens.apply(tokens, weight, scale, padding_idx, flag)
     return _lookup(tokens, weight, scale, flag)
+
+
+# embed_tokens as an operator of torch's own, for torch.jit.trace: its graph calls back here (whoever loads one imports this package)
+_library = torch.library.Library("diffsvc_amd", "DEF")
+_library.define("embed_tokens(Tensor tokens, Tensor weight, float scale, int? padding_idx, Tensor(a!)? flag) -> Tensor")
+_library.impl("embed_tokens", embed_tokens, "CompositeImplicitAutograd")
 
 
 class TokenEmbeddingHip(nn.Embedding):

@@ -1,4 +1,4 @@
-"""The lookup under torch's transforms, against nn.functional.embedding under the same: forward-mode derivatives.  On the device, and on the
+"""The lookup under torch's transforms, against nn.functional.embedding under the same: forward-mode derivatives, traces.  On the device, and on the
 host with the two kernel launches replaced by numpy -- code that no transform can look into, as the kernels are."""
 import numpy as np
 import pytest
@@ -66,6 +66,60 @@ def test_forward_mode(dev, grad, mode):
     if grad and mode:
         got.primal.sum().backward()
         assert not w.grad[PAD].any() and w.grad.any()
+
+
+@pytest.mark.parametrize("trained", [False, True])
+def test_trace(dev, trained, tmp_path):
+    """A traced lookup is the lookup, on tokens, tables and shapes that it was not traced on, with its gradient and its flag, saved and loaded too."""
+    w, t = small(V, H, dev=dev).requires_grad_(trained), tokens(dev, 4, 5)
+    flag = torch.zeros(1, dtype=torch.int32, device=dev)
+    traced = torch.jit.trace(lambda a, b, c: ours(a, b, c) + 1, (t, w, flag))
+    torch.jit.save(traced, str(tmp_path / "t.pt"))
+    w2, t2 = small(V, H, seed=5, dev=dev), tokens(dev, 9, seed=6)
+    for f in (traced, torch.jit.load(str(tmp_path / "t.pt"))):
+        assert "embed_tokens" in str(f.graph)
+        for _ in range(3):                                                 # (the executor looks at the first runs before it settles)
+            x = w2.clone().requires_grad_(True)
+            y = f(t2, x, flag)
+            assert torch.equal(y, plain(t2, w2) + 1)
+            y.sum().backward()
+            z = w2.clone().requires_grad_(True)
+            plain(t2, z).sum().backward()
+            assert torch.equal(x.grad, z.grad) and not flag.any()
+        with torch.no_grad():
+            assert torch.equal(f(t2, w2, flag), plain(t2, w2) + 1)
+        f(torch.full_like(t2, V), w2, flag)
+        assert flag.item() == 1
+        flag.zero_()
+
+
+def test_trace_refuses_what_the_call_refuses(dev):
+    w, t = small(V, H, dev=dev), tokens(dev, 4)
+    with pytest.raises(ValueError, match="padding_idx"):
+        torch.jit.trace(lambda a, b: T.embed_tokens(a, b, 1.0, V), (t, w))
+
+
+@pytest.mark.gpu
+def test_other_calls_refuse_to_be_traced():
+    from diffsvc_amd import muon
+    x, t = small(V, H, dev="cuda"), tokens("cuda", V)
+    for f, a in ((muon.orthogonalize, (x,)), (lambda t, d: T.embed_tokens_grad(t, d, V), (t, x))):
+        with pytest.raises(RuntimeError, match="a trace would record"):
+            torch.jit.trace(f, a)
+
+
+@pytest.mark.gpu
+def test_trace_of_the_module():
+    m = T.TokenEmbeddingHip(V, H, padding_idx=PAD, scale=SCALE).cuda()
+    with torch.no_grad():
+        f = torch.jit.trace(m, (tokens("cuda", 6),))
+    m.weight.data.copy_(small(V, H, dev="cuda"))
+    t = tokens("cuda", 3, 2, seed=9)
+    assert torch.equal(f(t), plain(t, m.weight)) and torch.equal(f(t), m(t))
+    m.check()
+    f(torch.tensor([V], device="cuda"))
+    with pytest.raises(IndexError):
+        m.check()
 
 
 @pytest.mark.gpu
