@@ -114,14 +114,38 @@ class _EmbedTokens(torch.autograd.Function):
         ctx.args = weight.shape[0], scale, padding_idx
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        vocab, scale, padding_idx = ctx.args
-        return None, embed_tokens_grad(ctx.saved_tensors[0], dy, vocab, scale, padding_idx), None, None, None
+        graph = torch.is_grad_enabled() or forward_ad._current_level >= 0          # (create_graph, or a tangent of dy)
+        return None, (_EmbedTokensGrad.apply if graph else embed_tokens_grad)(ctx.saved_tensors[0], dy, *ctx.args), None, None, None
 
     @staticmethod
     def jvp(ctx, _, dw, *__):                      # linear in the table; its row padding_idx counts forwards, as in nn.Embedding
         return _EmbedTokens.apply(ctx.saved_tensors[0], dw, ctx.args[1], ctx.args[2], None)
+
+
+class _EmbedTokensGrad(torch.autograd.Function):
+    """embed_tokens_grad as a linear map of dy: its own backward pass is the lookup without the places of padding_idx."""
+
+    @staticmethod
+    def forward(tokens, dy, vocab, scale, padding_idx):
+        return embed_tokens_grad(tokens, dy, vocab, scale, padding_idx)
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        tokens, _, *ctx.args = inputs
+        ctx.save_for_backward(tokens)
+        ctx.save_for_forward(tokens)
+
+    @staticmethod
+    def backward(ctx, dw):
+        (tokens,), (_, scale, padding_idx) = ctx.saved_tensors, ctx.args
+        if padding_idx is not None:
+            tokens = torch.where(tokens == padding_idx, -1, tokens)
+        return None, embed_tokens(tokens, dw, scale), None, None, None
+
+    @staticmethod
+    def jvp(ctx, _, d_dy, *__):
+        return _EmbedTokensGrad.apply(ctx.saved_tensors[0], d_dy, *ctx.args)
 
 
 def embed_tokens(tokens, weight, scale=1.0, padding_idx=None, flag=None):

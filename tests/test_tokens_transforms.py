@@ -1,4 +1,4 @@
-"""The lookup under torch's transforms, against nn.functional.embedding under the same: forward-mode derivatives, traces.  On the device, and on the
+"""The lookup under torch's transforms, against nn.functional.embedding under the same: forward-mode derivatives, traces, derivatives of derivatives.  On the device, and on the
 host with the two kernel launches replaced by numpy -- code that no transform can look into, as the kernels are."""
 import numpy as np
 import pytest
@@ -66,6 +66,27 @@ def test_forward_mode(dev, grad, mode):
     if grad and mode:
         got.primal.sum().backward()
         assert not w.grad[PAD].any() and w.grad.any()
+
+
+def test_derivatives_of_derivatives(dev):
+    """d/dr of <dW(r), D> is the lookup of D without the padding's places; the gradient of a gradient's square; forward over backward."""
+    t, r0, D = tokens(dev, 4, 5), small(4, 5, H, seed=3, dev=dev), small(V, H, seed=4, dev=dev)
+    assert (t == PAD).any()
+    res = []
+    for f in (ours, plain):
+        w, r = small(V, H, dev=dev).requires_grad_(True), r0.clone().requires_grad_(True)
+        dw, = torch.autograd.grad((f(t, w) * r).sum(), w, create_graph=True)
+        first = torch.autograd.grad((dw * D).sum(), r, retain_graph=True)[0]
+        second = torch.autograd.grad((dw * dw).sum(), r, create_graph=True)[0]
+        third = torch.autograd.grad((second * second).sum(), r)[0]
+        d2 = torch.autograd.grad(((f(t, w) ** 2).sum()), w, create_graph=True)[0]
+        hvp = torch.autograd.grad((d2 * D).sum(), w)[0]
+        with fw.dual_level():
+            x = fw.make_dual(w.detach().clone().requires_grad_(True), D)
+            jg = fw.unpack_dual(torch.autograd.grad((f(t, x) ** 2).sum(), x, create_graph=True)[0]).tangent
+        res.append((dw, first, second, third, d2, hvp, jg))
+    for a, b in zip(*res):
+        assert torch.equal(a, b) and b.any()
 
 
 @pytest.mark.parametrize("trained", [False, True])
