@@ -18,11 +18,12 @@ from . import _lib
 from ._lib import check, lib
 
 DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_tracing = torch._C._get_tracing_state
 
 
 def launch(t, fn, *args):
     """fn(*args, stream) on t's device and that device's current stream; raises what the library reports."""
-    if torch._C._get_tracing_state() is not None:
+    if _tracing() is not None:
         raise RuntimeError("diffsvc_amd: a trace would record the memory of this call without the kernels that fill it")
     i = t.device.index
     if i == torch._C._cuda_getDevice():
@@ -101,7 +102,40 @@ def embed_tokens_grad(tokens, dy, vocab, scale=1.0, padding_idx=None, out=None, 
     return out
 
 
+# torch.func wants a function's forward and setup_context apart, at 15 us of host time a call: it has subclasses of its own (.func)
+_func_active = torch._C._are_functorch_transforms_active
+
+
+def _apply(f, *args):
+    return (f.func if _func_active() else f).apply(*args)
+
+
+def _each(f, info, in_dims, *args):
+    """vmap by hand: f on every slice of the batched arguments."""
+    return torch.stack([_apply(f, *(a if d is None else a.select(d, i) for a, d in zip(args, in_dims))) for i in range(info.batch_size)]), 0
+
+
 class _EmbedTokens(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, tokens, weight, scale, padding_idx, flag):
+        ctx.save_for_backward(tokens)
+        ctx.save_for_forward(tokens)
+        ctx.args = weight.shape[0], scale, padding_idx
+        return _lookup(tokens, weight, scale, flag)
+
+    @staticmethod
+    def backward(ctx, dy):
+        args = (ctx.saved_tensors[0], dy, *ctx.args)
+        if torch.is_grad_enabled() or forward_ad._current_level >= 0 or _func_active():      # (create_graph, or a dy with a tangent or a batch)
+            return None, _apply(_EmbedTokensGrad, *args), None, None, None
+        return None, embed_tokens_grad(*args), None, None, None
+
+    @staticmethod
+    def jvp(ctx, _, dw, *__):                      # linear in the table; its row padding_idx counts forwards, as in nn.Embedding
+        return _apply(_EmbedTokens, ctx.saved_tensors[0], dw, ctx.args[1], ctx.args[2], None)
+
+
+class _EmbedTokensFunc(_EmbedTokens):
     @staticmethod
     def forward(tokens, weight, scale, padding_idx, flag):
         return _lookup(tokens, weight, scale, flag)
@@ -114,18 +148,38 @@ class _EmbedTokens(torch.autograd.Function):
         ctx.args = weight.shape[0], scale, padding_idx
 
     @staticmethod
-    def backward(ctx, dy):
-        graph = torch.is_grad_enabled() or forward_ad._current_level >= 0          # (create_graph, or a tangent of dy)
-        return None, (_EmbedTokensGrad.apply if graph else embed_tokens_grad)(ctx.saved_tensors[0], dy, *ctx.args), None, None, None
+    def vmap(info, in_dims, tokens, weight, *rest):
+        if in_dims[1] is None:                     # one table: the batch is one more dimension of the tokens
+            return _apply(_EmbedTokens, tokens.movedim(in_dims[0], 0), weight, *rest), 0
+        return _each(_EmbedTokens, info, in_dims, tokens, weight, *rest)
 
-    @staticmethod
-    def jvp(ctx, _, dw, *__):                      # linear in the table; its row padding_idx counts forwards, as in nn.Embedding
-        return _EmbedTokens.apply(ctx.saved_tensors[0], dw, ctx.args[1], ctx.args[2], None)
+
+_EmbedTokens.func = _EmbedTokensFunc
 
 
 class _EmbedTokensGrad(torch.autograd.Function):
     """embed_tokens_grad as a linear map of dy: its own backward pass is the lookup without the places of padding_idx."""
 
+    @staticmethod
+    def forward(ctx, tokens, dy, *args):
+        ctx.save_for_backward(tokens)
+        ctx.save_for_forward(tokens)
+        ctx.args = args
+        return embed_tokens_grad(tokens, dy, *args)
+
+    @staticmethod
+    def backward(ctx, dw):
+        (tokens,), (_, scale, padding_idx) = ctx.saved_tensors, ctx.args
+        if padding_idx is not None:
+            tokens = torch.where(tokens == padding_idx, -1, tokens)
+        return None, embed_tokens(tokens, dw, scale), None, None, None
+
+    @staticmethod
+    def jvp(ctx, _, d_dy, *__):
+        return _apply(_EmbedTokensGrad, ctx.saved_tensors[0], d_dy, *ctx.args)
+
+
+class _EmbedTokensGradFunc(_EmbedTokensGrad):
     @staticmethod
     def forward(tokens, dy, vocab, scale, padding_idx):
         return embed_tokens_grad(tokens, dy, vocab, scale, padding_idx)
@@ -137,30 +191,26 @@ class _EmbedTokensGrad(torch.autograd.Function):
         ctx.save_for_forward(tokens)
 
     @staticmethod
-    def backward(ctx, dw):
-        (tokens,), (_, scale, padding_idx) = ctx.saved_tensors, ctx.args
-        if padding_idx is not None:
-            tokens = torch.where(tokens == padding_idx, -1, tokens)
-        return None, embed_tokens(tokens, dw, scale), None, None, None
+    def vmap(info, in_dims, *args):
+        return _each(_EmbedTokensGrad, info, in_dims, *args)
 
-    @staticmethod
-    def jvp(ctx, _, d_dy, *__):
-        return _EmbedTokensGrad.apply(ctx.saved_tensors[0], d_dy, *ctx.args)
+
+_EmbedTokensGrad.func = _EmbedTokensGradFunc
 
 
 def embed_tokens(tokens, weight, scale=1.0, padding_idx=None, flag=None):
     """scale * weight[tokens], [..., H] for tokens [...]; differentiable in ``weight`` (backwards and forwards), whose row ``padding_idx`` gets no gradient.
     flag: an int32 device tensor that is set to 1 where a token lies outside the table (its row is zero)."""
     scale = float(scale)
-    if torch._C._get_tracing_state() is not None:                  # a trace sees no kernel launch: it records the operator
+    if _tracing() is not None:                                     # a trace sees no kernel launch: it records the operator
         return torch.ops.diffsvc_amd.embed_tokens(tokens, weight, scale, padding_idx, flag)
     if padding_idx is not None:
         padding_idx = _padding(padding_idx, weight.shape[0])
     if flag is not None and (flag.dtype != torch.int32 or flag.device != weight.device or flag.numel() < 1):
         raise ValueError("flag must be an int32 tensor on %s" % weight.device)
     # (a table that takes no gradient and has no tangent has no use for the graph)
-    if weight.requires_grad and torch.is_grad_enabled() or forward_ad._current_level >= 0:
-        return _EmbedTokens.apply(tokens, weight, scale, padding_idx, flag)
+    if weight.requires_grad and torch.is_grad_enabled() or forward_ad._current_level >= 0 or _func_active():
+        return _apply(_EmbedTokens, tokens, weight, scale, padding_idx, flag)
     return _lookup(tokens, weight, scale, flag)
 
 

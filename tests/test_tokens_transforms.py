@@ -1,4 +1,5 @@
-"""The lookup under torch's transforms, against nn.functional.embedding under the same: forward-mode derivatives, traces, derivatives of derivatives.  On the device, and on the
+"""The lookup under torch's transforms, against nn.functional.embedding under the same: forward-mode derivatives, traces, derivatives of derivatives, torch.func.
+On the device, and on the
 host with the two kernel launches replaced by numpy -- code that no transform can look into, as the kernels are."""
 import numpy as np
 import pytest
@@ -87,6 +88,23 @@ def test_derivatives_of_derivatives(dev):
         res.append((dw, first, second, third, d2, hvp, jg))
     for a, b in zip(*res):
         assert torch.equal(a, b) and b.any()
+
+
+def test_func_transforms(dev):
+    t, tb, w, wb = tokens(dev, 6), tokens(dev, 3, 6, seed=7), small(V, H, dev=dev), small(3, V, H, seed=8, dev=dev)
+    assert (tb == PAD).any()
+    f = torch.func
+    loss = lambda g: lambda t, w: (g(t, w) ** 2).sum()
+    calls = [lambda g: f.vmap(g, (0, None))(tb, w), lambda g: f.vmap(g, (None, 0))(t, wb), lambda g: f.vmap(g, (0, 0))(tb, wb), lambda g: f.vmap(g, (1, 2))(tb.t(), wb.permute(1, 2, 0)),
+             lambda g: f.vmap(f.vmap(g, (0, None)), (None, 0))(tb, wb), lambda g: f.grad(loss(g), 1)(t, w), lambda g: f.vmap(f.grad(loss(g), 1), (0, None))(tb, w),
+             lambda g: f.vmap(f.grad(loss(g), 1), (0, 0))(tb, wb), lambda g: f.jvp(lambda x: g(t, x), (w,), (wb[0],))[1], lambda g: f.vjp(lambda x: g(t, x), w)[1](small(6, H, seed=9, dev=dev))[0],
+             lambda g: f.jacrev(g, 1)(t[:2], w), lambda g: f.jacfwd(g, 1)(t[:2], w), lambda g: f.hessian(loss(g), 1)(t[:3], w[:, :2].contiguous()),
+             lambda g: f.jvp(f.grad(lambda x: loss(g)(t, x)), (w,), (wb[1],))[1]]
+    for i, c in enumerate(calls):
+        a, b = c(ours), c(plain)
+        assert a.shape == b.shape and torch.equal(a, b) and b.any(), i
+    with torch.no_grad():
+        assert torch.equal(f.vmap(ours, (0, None))(tb, w), plain(tb, w))
 
 
 @pytest.mark.parametrize("trained", [False, True])
