@@ -299,7 +299,7 @@ class DiffusionTrainerHip:
             self.grads.mul_(1.0 / world)
         return loss
 
-    CHECK_EVERY = 100              # optimiser steps between two reads of the trainer's sticky argument flag (dsvc_trainer_check synchronises)
+    CHECK_EVERY = 100              # optimiser steps between two reads of the sticky argument flags (dsvc_trainer_check synchronises)
 
     @torch.no_grad()
     def train_step(self, hubert, mel2ph, f0, mels, t=None, seed=None, first_clip=0, clip_ids=None, overlap=None, energy=None):
@@ -332,6 +332,8 @@ class DiffusionTrainerHip:
         self.global_step += 1
         if self.global_step % self.CHECK_EVERY == 0:
             self.h.check()                                   # the trainer's sticky "diffusion step outside the schedule" flag: one sync per 100 steps
+            if self.energy_vocab:
+                self.fs2.energy_embed.check()                # and the energy table's: a frame energy below zero has no row
         hp, n = self.hp, self.n_floats
         clip = float(hp.get("clip_grad_norm", 1.0))
         coef = None
