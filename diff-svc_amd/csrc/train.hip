@@ -1739,7 +1739,15 @@ int dsvc_trainer_step(dsvc_trainer* t, const dsvc_train_args* a, float* loss_out
     if (!t->params || !t->grads) return fail(DSVC_ESTATE, "trainer: bind the flat parameter / gradient buffers first");
     if (!t->sa.p) return fail(DSVC_ESTATE, "trainer: set the noise schedule first");
     if (a->B < 1 || a->T < 1 || (a->T * t->cfg.mel_bins) % 4) return fail(DSVC_EINVAL, "trainer: bad batch geometry");
-    return t->step(a, loss_out, (hipStream_t)stream);
+    const int rc = t->step(a, loss_out, (hipStream_t)stream);
+    if (rc != DSVC_OK) t->next_layer = -1;           // a step that failed is over: it leaves no phase open
+    return rc;
+}
+
+int dsvc_trainer_abandon(dsvc_trainer* t) {
+    if (!t) return fail(DSVC_EINVAL, "null handle");
+    t->next_layer = -1;
+    return DSVC_OK;
 }
 
 int dsvc_adamw_step(float* params, const float* grads, float* exp_avg, float* exp_avg_sq, int64_t n, float lr, float beta1, float beta2,

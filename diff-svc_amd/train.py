@@ -87,8 +87,15 @@ class TrainerHandle:
         self._ck(self._L.dsvc_trainer_set_cond_grad(self._h, None if g is None else g.data_ptr(), 0 if g is None else g.shape[0] * g.shape[1]))
         self._cond_grad = g
 
+    def _abandon(self):
+        """A step that was begun and not ended (an exception between its phases) is given up: a new one begins."""
+        if self._inflight is not None:
+            self._ck(self._L.dsvc_trainer_abandon(self._h))
+            self._inflight = None
+
     def step(self, mel, cond, t, pitch=None, mel2ph=None, seed=0, first_clip=0, clip_ids=None, loss_out=None, cond_grad=None):
         """cond_grad: a float32 [B, T, H] tensor that gets d loss / d cond, transposed (None: not computed)."""
+        self._abandon()
         a, keep = self._args(mel, cond, t, pitch, mel2ph, seed, first_clip, clip_ids)
         loss = loss_out if loss_out is not None else torch.empty(1, device=mel.device, dtype=torch.float32)
         self._want_cond_grad(cond_grad, mel)
@@ -100,6 +107,7 @@ class TrainerHandle:
 
     # the same step in phases (include/dsvc.h): after each call a contiguous slice of the gradient buffer is final
     def step_begin(self, mel, cond, t, pitch=None, mel2ph=None, seed=0, first_clip=0, clip_ids=None, cond_grad=None):
+        self._abandon()
         a, self._inflight = self._args(mel, cond, t, pitch, mel2ph, seed, first_clip, clip_ids)
         self._want_cond_grad(cond_grad, mel)
         self._ck(self._L.dsvc_trainer_step_begin(self._h, ctypes.byref(a), stream_ptr()))

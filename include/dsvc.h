@@ -369,6 +369,9 @@ DSVC_API int dsvc_trainer_step_begin(dsvc_trainer* t, const dsvc_train_args* a, 
 DSVC_API int dsvc_trainer_check(dsvc_trainer* t, void* stream);
 DSVC_API int dsvc_trainer_step_layers(dsvc_trainer* t, int32_t l_hi, int32_t l_lo, void* stream);
 DSVC_API int dsvc_trainer_step_end(dsvc_trainer* t, float* loss_out, void* stream);
+/* gives up the step in flight, if there is one: its gradients are undefined, and whatever waits for its end (dsvc_trainer_set_cond_grad) may be
+ * called again.  A dsvc_trainer_step that failed needs no such call. */
+DSVC_API int dsvc_trainer_abandon(dsvc_trainer* t);
 /* torch.optim.AdamW update of a flat buffer.  The gradient is multiplied by *grad_scale_dev (device, e.g. the clip coefficient)
  * when that pointer is not NULL, else by grad_scale. */
 DSVC_API int dsvc_adamw_step(float* params, const float* grads, float* exp_avg, float* exp_avg_sq, int64_t n, float lr, float beta1, float beta2,
