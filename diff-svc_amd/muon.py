@@ -16,7 +16,7 @@ import torch
 
 from . import _lib
 from ._lib import check, lib
-from .tokens import DTYPES, launch
+from .tokens import DTYPES, launch, refuse_trace
 
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 PLANES = {None: 0, "f16": 1, "f16_x3": 2}
@@ -77,6 +77,7 @@ def _workspace(L, cfg, t):
 @torch.no_grad()
 def orthogonalize(x, steps=5, coefficients=COEFFICIENTS, eps=1e-7, scale=1.0, precision=None, out=None):
     """scale * the Newton-Schulz iterate of every matrix of x [..., rows, cols], in x's type.  ``out`` may be x itself."""
+    refuse_trace()
     _check("x", x)
     v = _matrices("x", x, True)
     if out is None:
@@ -103,6 +104,7 @@ def muon_step_(param, grad, momentum_buffer, lr, momentum=0.95, nesterov=True, w
 
     momentum_buffer is float32; grad has param's type; the three do not overlap.  grad_scale: a number or a one-element float32 device tensor (a
     clip coefficient)."""
+    refuse_trace()
     _check("param", param)
     if grad.shape != param.shape or grad.dtype != param.dtype or grad.device != param.device:
         raise ValueError("grad must be %s %s on %s" % (tuple(param.shape), param.dtype, param.device))

@@ -18,13 +18,11 @@ from . import _lib
 from ._lib import check, lib
 
 DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-_tracing = torch._C._get_tracing_state
+_tracing = torch._C._is_tracing
 
 
 def launch(t, fn, *args):
     """fn(*args, stream) on t's device and that device's current stream; raises what the library reports."""
-    if _tracing() is not None:
-        raise RuntimeError("diffsvc_amd: a trace would record the memory of this call without the kernels that fill it")
     i = t.device.index
     if i == torch._C._cuda_getDevice():
         rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
@@ -33,6 +31,11 @@ def launch(t, fn, *args):
             rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
     if rc:
         check(rc)
+
+
+def refuse_trace():
+    if _tracing():
+        raise RuntimeError("diffsvc_amd: a trace would record the memory of this call without the kernels that fill it")
 
 
 def rows_of(t):
@@ -74,6 +77,7 @@ def _lookup(tokens, weight, scale, flag):
 def embed_tokens_grad(tokens, dy, vocab, scale=1.0, padding_idx=None, out=None, accumulate=False):
     """Gradient of ``embed_tokens`` in its table, [vocab, H]: dy is [..., H] over tokens of shape [...].  ``out`` (dy's type or float32) is
     written whole, zeros where a token does not occur; with ``accumulate`` the sums are added to what it holds instead.  It does not overlap dy."""
+    refuse_trace()
     if dy.dtype not in DTYPES:
         raise TypeError("diffsvc_amd: gradients are float32, float16 or bfloat16, got %s" % dy.dtype)
     if dy.dim() < 1 or tuple(dy.shape[:-1]) != tuple(tokens.shape) or not dy.shape[-1]:
@@ -202,7 +206,7 @@ def embed_tokens(tokens, weight, scale=1.0, padding_idx=None, flag=None):
     """scale * weight[tokens], [..., H] for tokens [...]; differentiable in ``weight`` (backwards and forwards), whose row ``padding_idx`` gets no gradient.
     flag: an int32 device tensor that is set to 1 where a token lies outside the table (its row is zero)."""
     scale = float(scale)
-    if _tracing() is not None:                                     # a trace sees no kernel launch: it records the operator
+    if _tracing():                                                 # a trace sees no kernel launch: it records the operator
         return torch.ops.diffsvc_amd.embed_tokens(tokens, weight, scale, padding_idx, flag)
     if padding_idx is not None:
         padding_idx = _padding(padding_idx, weight.shape[0])
