@@ -283,6 +283,7 @@ __global__ __launch_bounds__(256) void k_sort_scatter(SortSrc s, long long n, in
 // ---- 2. chunks of sorted places --------------------------------------------------------------------------------------------------------------
 // Bound by memory: 32768 places of 2048 bf16 columns and a table of 50000 rows take 73 us (339 MB, 4.7 TB/s: a large copy's rate).  Eight rows are in
 // flight per wave, since a gathered row's latency is all there is to hide.  8192 fp32 rows of 256 columns onto 256 rows: 6 us.
+constexpr long long MAX_WAVES = 1 << 25;     // a launch's share of each kind of work: 2^26 waves of 64 are more than a grid may hold
 constexpr int ZERO_ROWS = 16, ZERO_SLICES = 4;   // rows of dW that one wave looks up and zeroes, and slices of them (a wave for whole rows: 45 rows of 4245
                                              // columns take 25 us, when two places are all there is to add)
 
@@ -354,29 +355,32 @@ __global__ __launch_bounds__(256) void k_seg_sum(const SegArgs a) {
     const int lane = threadIdx.x & 63;
     const long long unit = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n_seg = a.n_chunks * a.slices;
     if (unit >= n_seg) {                     // zero the rows that no place belongs to
+        if (a.accumulate) return;
         const int groups = (a.slices + ZERO_SLICES - 1) / ZERO_SLICES;
-        const long long z = (unit - n_seg) / groups, v0 = z * ZERO_ROWS;
-        const int s0 = (int)(unit - n_seg - z * groups) * ZERO_SLICES, s1 = s0 + ZERO_SLICES < a.slices ? s0 + ZERO_SLICES : a.slices;
-        if (a.accumulate || v0 >= a.V) return;
-        bool absent = false;
-        if (lane < ZERO_ROWS && v0 + lane < a.V) {
-            const unsigned v = (unsigned)(v0 + lane);
-            long long lo = 0, hi = a.n;      // first place whose key is not below v
-            while (lo < hi) {
-                const long long mid = (lo + hi) >> 1;
-                if (a.keys[mid] < v) lo = mid + 1; else hi = mid;
+        const long long units = (a.V + ZERO_ROWS - 1ll) / ZERO_ROWS * groups, waves = gridDim.x * 4ll - n_seg;
+        for (long long u = unit - n_seg; u < units; u += waves) {        // (once, up to MAX_WAVES of them)
+            const long long z = u / groups, v0 = z * ZERO_ROWS;
+            const int s0 = (int)(u - z * groups) * ZERO_SLICES, s1 = s0 + ZERO_SLICES < a.slices ? s0 + ZERO_SLICES : a.slices;
+            bool absent = false;
+            if (lane < ZERO_ROWS && v0 + lane < a.V) {
+                const unsigned v = (unsigned)(v0 + lane);
+                long long lo = 0, hi = a.n;  // first place whose key is not below v
+                while (lo < hi) {
+                    const long long mid = (lo + hi) >> 1;
+                    if (a.keys[mid] < v) lo = mid + 1; else hi = mid;
+                }
+                absent = lo >= a.n || a.keys[lo] != v;
             }
-            absent = lo >= a.n || a.keys[lo] != v;
-        }
-        unsigned long long todo = __ballot(absent);
-        float zero[VEC];
+            unsigned long long todo = __ballot(absent);
+            float zero[VEC];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) zero[e] = 0.f;
-        while (todo) {
-            const int r = __ffsll((long long)todo) - 1;
-            todo &= todo - 1;
-            O* p = (O*)a.dw + (v0 + r) * a.dw_ld;
-            for (int s = s0; s < s1; ++s) store_row<O, VEC, VECTOR>(p, s * 64 * VEC + (VECTOR ? lane * VEC : lane), a.H, zero);
+            for (int e = 0; e < VEC; ++e) zero[e] = 0.f;
+            while (todo) {
+                const int r = __ffsll((long long)todo) - 1;
+                todo &= todo - 1;
+                O* p = (O*)a.dw + (v0 + r) * a.dw_ld;
+                for (int s = s0; s < s1; ++s) store_row<O, VEC, VECTOR>(p, s * 64 * VEC + (VECTOR ? lane * VEC : lane), a.H, zero);
+            }
         }
         return;
     }
@@ -508,6 +512,7 @@ int grad_plan(int64_t n, int64_t V, int32_t H, int esize, GradPlan* p) {
     const long long want = n * slices / 4096;
     p->chunk = (int)(want < 2 ? 8 : want < 16 ? 16 : want > 2048 ? 2048 : (want + 7) / 8 * 8);
     p->n_chunks = (n + p->chunk - 1) / p->chunk;
+    if (p->n_chunks * ((H + 255) / 256) > MAX_WAVES) return fail(DSVC_EINVAL, "embed_tokens_grad: %lld tokens of %d columns are too many", (long long)n, H);
     p->blocks = (n + 256 * p->ipt - 1) / (256 * p->ipt);
     long long at = 0;
     auto take = [&](long long bytes) { const long long o = at; at += (bytes + 255) / 256 * 256; return o; };
@@ -550,8 +555,8 @@ int sort_many(const void* tokens, int i64, long long n, long long V, long long p
 template <int TD, int TO, int VEC, bool VECTOR>
 int segments(SegArgs a, hipStream_t st) {
     a.slices = ceil_div(a.H, 64 * VEC);
-    const long long zero = a.accumulate ? 0 : (((long long)a.V + ZERO_ROWS - 1) / ZERO_ROWS) * ceil_div(a.slices, ZERO_SLICES), units = a.n_chunks * a.slices + zero;
-    if (units >= (1LL << 26)) return fail(DSVC_EINVAL, "embed_tokens_grad: %lld work items", units);
+    const long long all = a.accumulate ? 0 : (((long long)a.V + ZERO_ROWS - 1) / ZERO_ROWS) * ceil_div(a.slices, ZERO_SLICES), zero = all < MAX_WAVES - 4 ? all : MAX_WAVES - 4;
+    const long long units = a.n_chunks * a.slices + zero;        // (at most MAX_WAVES of the first: grad_plan)
     if (units) hipLaunchKernelGGL((k_seg_sum<TD, TO, VEC, VECTOR>), dim3((unsigned)((units + 3) / 4)), dim3(256), 0, st, a);
     if (a.n_chunks > 1) hipLaunchKernelGGL((k_seg_join<TO, VEC, VECTOR>), dim3((unsigned)(a.n_chunks - 1), a.slices), dim3(JOIN_WAVES * 64), 0, st, a);
     DSVC_HIP(hipGetLastError());

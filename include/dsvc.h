@@ -398,7 +398,8 @@ DSVC_API int dsvc_embed_tokens(const void* tokens, int32_t tokens_i64, int64_t n
                                float scale, void* out, int64_t out_ld, int32_t* out_of_range, void* stream);
 /* dw[v] (+)= scale * sum of dy[i] over the places i with tokens[i] == v, in fp32 in a fixed order (bit-identical from call to call), rounded once;
  * accumulate == 0 overwrites all vocab rows (zeros where a token does not occur), else adds to the rows that occur.  padding_idx (a negative
- * value: none) and tokens outside [0, vocab) contribute nothing.  dw has dy's type or fp32. */
+ * value: none) and tokens outside [0, vocab) contribute nothing.  dw has dy's type or fp32.  Up to 2^28 tokens, 2^30 rows and 2^20 columns, and 2^44 elements of
+ * dy; the workspace query refuses what the call refuses. */
 DSVC_API int dsvc_embed_tokens_grad_workspace(int64_t n, int64_t vocab, int32_t H, int64_t* bytes);
 DSVC_API int dsvc_embed_tokens_grad(const void* tokens, int32_t tokens_i64, int64_t n, const void* dy, int64_t dy_ld, int32_t dy_dtype, int64_t vocab, int32_t H,
                                     float scale, int64_t padding_idx, void* dw, int64_t dw_ld, int32_t dw_dtype, int32_t accumulate, void* workspace,

@@ -254,3 +254,16 @@ def test_module_captured_with_its_backward_pass():
     with pytest.raises(IndexError):
         m.check()
     assert list(m.state_dict()) == ["weight"]
+
+
+@pytest.mark.parametrize("V", [1 << 30, (1 << 30) - 15])
+def test_gradient_of_a_table_with_the_most_rows(V):
+    """2^30 rows: more rows to zero than one launch has waves for."""
+    t = torch.tensor([V - 1, 5, V - 1, V - 17, V, 1 << 29], device="cuda")
+    dy = torch.arange(1, 7, device="cuda", dtype=torch.float32)[:, None].bfloat16()
+    out = torch.full((V, 1), 9.0, device="cuda", dtype=torch.bfloat16)
+    T.embed_tokens_grad(t, dy, V, out=out)
+    assert [out[i, 0].item() for i in (V - 1, 5, V - 17, 1 << 29)] == [4, 2, 4, 6]
+    assert int(torch.count_nonzero(out)) == 4
+    T.embed_tokens_grad(t[:2], dy[:2], V, out=out, accumulate=True)
+    assert out[V - 1, 0].item() == 5 and out[5, 0].item() == 4 and int(torch.count_nonzero(out)) == 4

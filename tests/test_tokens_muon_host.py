@@ -151,3 +151,15 @@ def test_module_on_the_host_is_the_plain_embedding():
     with pytest.raises(NotImplementedError):
         tokens.TokenEmbeddingHip(7, 5, sparse=True)
     assert muon.rms_scale(4, 25) == pytest.approx(1.0)
+
+
+def test_embedding_gradients_are_refused_before_anything_runs():
+    """The workspace query and the call refuse the same sizes: none gets past the query and fails after its first launches."""
+    L, n = _lib.lib(), ctypes.c_int64(-1)
+    for N, V, H in ((1 << 28, 10, 1 << 20), (1 << 25, 10, 1 << 20), (1 << 28, 1 << 30, 1 << 17)):
+        refused(L.dsvc_embed_tokens_grad_workspace(N, V, H, ctypes.byref(n)), "too many")
+        assert n.value == -1
+        for dt in (0, 1, 2):
+            refused(L.dsvc_embed_tokens_grad(P, 0, N, P, H, dt, V, H, 1.0, -1, P, H, dt, 0, P, 1 << 60, None), "too many")
+    for N, V, H in ((0, 1 << 30, 1), (1 << 28, 1 << 30, 1), (5, 1 << 30, 1 << 20), (1 << 24, 7, 1 << 20)):
+        assert L.dsvc_embed_tokens_grad_workspace(N, V, H, ctypes.byref(n)) == 0, (N, V, H)
