@@ -71,7 +71,7 @@ __global__ __launch_bounds__(256) void k_embed(const void* __restrict__ tokens, 
                 const long long i = i0 + r * ty + y;
                 if (i >= n) continue;
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) v[r][e] = (E)((float)v[r][e] * scale);
+                for (int e = 0; e < VEC; ++e) v[r][e] = (E)one_value((float)v[r][e] * scale);      // (left alone, fp16 element by element rounds the exact product)
                 *(EV*)(o + i * out_ld + c) = v[r];
             }
         }

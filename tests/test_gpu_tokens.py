@@ -267,3 +267,20 @@ def test_gradient_of_a_table_with_the_most_rows(V):
     assert int(torch.count_nonzero(out)) == 4
     T.embed_tokens_grad(t[:2], dy[:2], V, out=out, accumulate=True)
     assert out[V - 1, 0].item() == 5 and out[5, 0].item() == 4 and int(torch.count_nonzero(out)) == 4
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_lookup_rounds_the_float32_product_whatever_the_alignment(dtype):
+    """scale * value in float32, then one rounding: rows of 8 aligned columns, and the same rows element by element.  Among the scales are ones where
+    the exact product, rounded once, would be another fp16 number (a float32 product that lies on a tie)."""
+    m = (1 + torch.arange(1024) / 1024).half()
+    scales = [s for s in (float(np.float32(k ** 0.5)) for k in range(2, 400)) if ((m.double() * s).numpy().astype(np.float16) != (m.float() * s).half().numpy()).any()]
+    assert len(scales) >= 5
+    g = torch.Generator().manual_seed(3)
+    w = torch.cat([m.float().repeat(60), torch.randn(100, generator=g)]).to(dtype)[:61504].view(-1, 64).cuda()
+    t = torch.randperm(w.shape[0], generator=g).cuda()
+    wide = torch.zeros(w.shape[0], 65, device="cuda", dtype=dtype)
+    wide[:, 1:] = w
+    for scale in scales[:5] + [16.0, 0.1]:
+        want = (w[t].float() * float(np.float32(scale))).to(dtype)
+        assert torch.equal(T.embed_tokens(t, w, scale), want) and torch.equal(T.embed_tokens(t, wide[:, 1:], scale), want), scale
