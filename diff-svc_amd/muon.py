@@ -28,22 +28,17 @@ def rms_scale(rows, cols, rms=0.2):
     return rms * math.sqrt(max(rows, cols))
 
 
-_coefficients = {}                 # (a, b, c) -> the C array
+_Coefficients = ctypes.c_float * 3
 
 
 def _cfg(t, steps, coefficients, eps, scale, precision):
     planes = PLANES.get(precision, -1)
     if planes < 0:
         raise ValueError("precision must be one of %s, got %r" % ([k for k in PLANES if k], precision))
-    coef = _coefficients.get(coefficients) if type(coefficients) is tuple else None
-    if coef is None:
-        if len(coefficients) != 3:
-            raise ValueError("three coefficients, got %r" % (coefficients,))
-        coef = (ctypes.c_float * 3)(*coefficients)
-        if type(coefficients) is tuple and len(_coefficients) < 64:
-            _coefficients[coefficients] = coef
+    if len(coefficients) != 3:
+        raise ValueError("three coefficients, got %r" % (coefficients,))
     B, m, n = t.shape
-    return _lib.OrthoCfg(DTYPES[t.dtype], planes, B, m, n, steps, coef, eps, scale)
+    return _lib.OrthoCfg(DTYPES[t.dtype], planes, B, m, n, steps, _Coefficients(*coefficients), eps, scale)
 
 
 def _check(name, t):

@@ -163,3 +163,12 @@ def test_embedding_gradients_are_refused_before_anything_runs():
             refused(L.dsvc_embed_tokens_grad(P, 0, N, P, H, dt, V, H, 1.0, -1, P, H, dt, 0, P, 1 << 60, None), "too many")
     for N, V, H in ((0, 1 << 30, 1), (1 << 28, 1 << 30, 1), (5, 1 << 30, 1 << 20), (1 << 24, 7, 1 << 20)):
         assert L.dsvc_embed_tokens_grad_workspace(N, V, H, ctypes.byref(n)) == 0, (N, V, H)
+
+
+def test_coefficients_are_read_at_every_call():
+    """One-element tensors are numbers too, and may have changed since the last call."""
+    a, x = torch.tensor(1.5), torch.zeros(1, 2, 2)
+    coef = (a, -0.5, 0.0)
+    assert muon._cfg(x, 5, coef, 1e-7, 1.0, None).coef[0] == 1.5
+    a.fill_(1.25)
+    assert list(muon._cfg(x, 5, coef, 1e-7, 1.0, None).coef) == [1.25, -0.5, 0.0]
