@@ -13,6 +13,7 @@ import ctypes
 import math
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from ._lib import check, lib
@@ -71,7 +72,8 @@ def _workspace(L, cfg, t):
 
 @torch.no_grad()
 def orthogonalize(x, steps=5, coefficients=COEFFICIENTS, eps=1e-7, scale=1.0, precision=None, out=None):
-    """scale * the Newton-Schulz iterate of every matrix of x [..., rows, cols], in x's type.  ``out`` may be x itself."""
+    """scale * the Newton-Schulz iterate of every matrix of x [..., rows, cols], in x's type.  ``out`` may be x itself.  The result carries no autograd
+    graph: an update is made of gradients, it is not differentiated."""
     refuse_trace()
     _check("x", x)
     v = _matrices("x", x, True)
@@ -86,6 +88,7 @@ def orthogonalize(x, steps=5, coefficients=COEFFICIENTS, eps=1e-7, scale=1.0, pr
     L = lib()
     ws, size = _workspace(L, cfg, v)
     launch(v, L.dsvc_orthogonalize, ctypes.byref(cfg), v.data_ptr(), v.stride(1), v.stride(0), o.data_ptr(), o.stride(1), o.stride(0), ws.data_ptr(), size)
+    increment_version(out)             # (a graph that saved it must not use it unawares)
     return out
 
 
@@ -118,4 +121,5 @@ def muon_step_(param, grad, momentum_buffer, lr, momentum=0.95, nesterov=True, w
     ws, size = _workspace(L, cfg, p)
     launch(p, L.dsvc_muon_step, ctypes.byref(cfg), p.data_ptr(), p.stride(1), p.stride(0), g.data_ptr(), g.stride(1), g.stride(0), m.data_ptr(), m.stride(1),
            m.stride(0), lr, momentum, nesterov, weight_decay, dev_scale, num_scale, ws.data_ptr(), size)
+    increment_version((param, momentum_buffer))
     return param

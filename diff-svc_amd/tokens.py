@@ -13,6 +13,7 @@ import ctypes
 import torch
 from torch import nn
 from torch.autograd import forward_ad
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from ._lib import check, lib
@@ -76,7 +77,8 @@ def _lookup(tokens, weight, scale, flag):
 
 def embed_tokens_grad(tokens, dy, vocab, scale=1.0, padding_idx=None, out=None, accumulate=False):
     """Gradient of ``embed_tokens`` in its table, [vocab, H]: dy is [..., H] over tokens of shape [...].  ``out`` (dy's type or float32) is
-    written whole, zeros where a token does not occur; with ``accumulate`` the sums are added to what it holds instead.  It does not overlap dy."""
+    written whole, zeros where a token does not occur; with ``accumulate`` the sums are added to what it holds instead.  It does not overlap dy.
+    The result carries no autograd graph (``torch.autograd.grad`` of ``embed_tokens`` with ``create_graph`` gives one that does)."""
     refuse_trace()
     if dy.dtype not in DTYPES:
         raise TypeError("diffsvc_amd: gradients are float32, float16 or bfloat16, got %s" % dy.dtype)
@@ -97,6 +99,8 @@ def embed_tokens_grad(tokens, dy, vocab, scale=1.0, padding_idx=None, out=None, 
         raise ValueError("out must be [%d, %d] of %s or float32 on %s" % (vocab, H, d.dtype, d.device))
     elif (H > 1 and out.stride(1) != 1) or (vocab > 1 and out.stride(0) < H):
         raise ValueError("out needs rows of unit stride that do not overlap, got strides %s" % (out.stride(),))
+    else:
+        increment_version(out)             # (a graph that saved it must not use it unawares)
     L = lib()
     need = ctypes.c_int64(0)
     check(L.dsvc_embed_tokens_grad_workspace(n, vocab, H, ctypes.byref(need)))

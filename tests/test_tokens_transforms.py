@@ -172,3 +172,17 @@ def test_forward_mode_of_the_module(trained):
     with fw.dual_level():
         a, b = (torch.func.functional_call(x, {"weight": fw.make_dual(x.weight, dw)}, (t,)) for x in (m, e))
         assert torch.equal(fw.unpack_dual(a).tangent, fw.unpack_dual(b).tangent) and torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_a_graph_notices_what_is_written_in_place():
+    """A tensor that a graph has saved and one of the kernels has written since: backward refuses, as after torch's own in-place operations."""
+    from diffsvc_amd import muon
+    t, d = tokens("cuda", 6), small(6, H, dev="cuda")
+    for write in (lambda x, m: muon.muon_step_(x, d[:4], m, 0.1), lambda x, m: muon.muon_step_(m.clone(), d[:4], x, 0.1), lambda x, m: muon.orthogonalize(d[:4], out=x),
+                  lambda x, m: T.embed_tokens_grad(t % 4, d, 4, out=x), lambda x, m: muon.muon_step_(x[1:3], d[:2], m[1:3], 0.1)):
+        x, m, y = torch.ones(4, H, device="cuda"), torch.zeros(4, H, device="cuda"), torch.ones(4, H, device="cuda", requires_grad=True)
+        loss = (x * y).sum()
+        write(x, m)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
