@@ -1077,11 +1077,11 @@ int dsvc_trainer::repack(hipStream_t st) {
                                     H, 1, 1, 0});
         // W_o^T(c, k) = W_o[k][c]
         tpack_q.push_back(TPackDesc{P(q + "output_projection.weight"), t_out_rm.as<int>(), nullptr, oT_t.as<_Float16>() + (size_t)l * oT_halfs, 2 * C, 1, C2p, C / 32, 1, C, 1, 0});
-        // transposed conv: dxin[c] = sum_tap sum_o W_d[o][c][2 - tap] * dy[row + (tap-1)*d][o]
         // dcond[h] += sum_o W_c[o][h] dy[o]
         if (cond_grad)
             tpack_q.push_back(TPackDesc{P(q + "conditioner_projection.weight"), t_cond_rm.as<int>(), nullptr, cT_t.as<_Float16>() + (size_t)l * cT_halfs, 2 * C, 1, C2p,
                                         ceil_div(H, 32), 1, H, 1, 0});
+        // transposed conv: dxin[c] = sum_tap sum_o W_d[o][c][2 - tap] * dy[row + (tap-1)*d][o]
         tpack_q.push_back(TPackDesc{P(q + "dilated_conv.weight"), t_out_rm.as<int>(), nullptr, dT_t.as<_Float16>() + (size_t)l * dT_halfs, 2 * C, 3, C2p, C / 32, 3, (long long)C * 3, 1, 1});
     }
     return flush_packs(st);
