@@ -223,9 +223,10 @@ def embed_tokens(tokens, weight, scale=1.0, padding_idx=None, flag=None):
 
 
 # embed_tokens as an operator of torch's own, for torch.jit.trace: its graph calls back here (whoever loads one imports this package)
-_library = torch.library.Library("diffsvc_amd", "DEF")
-_library.define("embed_tokens(Tensor tokens, Tensor weight, float scale, int? padding_idx, Tensor(a!)? flag) -> Tensor")
-_library.impl("embed_tokens", embed_tokens, "CompositeImplicitAutograd")
+if not hasattr(torch.ops.diffsvc_amd, "embed_tokens"):              # (a module that is loaded again finds it)
+    _library = torch.library.Library("diffsvc_amd", "FRAGMENT")
+    _library.define("embed_tokens(Tensor tokens, Tensor weight, float scale, int? padding_idx, Tensor(a!)? flag) -> Tensor")
+    _library.impl("embed_tokens", embed_tokens, "CompositeImplicitAutograd")
 
 
 class TokenEmbeddingHip(nn.Embedding):

@@ -138,6 +138,14 @@ def test_trace_refuses_what_the_call_refuses(dev):
         torch.jit.trace(lambda a, b: T.embed_tokens(a, b, 1.0, V), (t, w))
 
 
+def test_the_module_may_be_loaded_again():
+    import os
+    import subprocess
+    import sys
+    code = "import importlib, diffsvc_amd; from diffsvc_amd import tokens; importlib.reload(tokens)"
+    subprocess.run([sys.executable, "-c", code], check=True, cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))), timeout=300)
+
+
 @pytest.mark.gpu
 def test_other_calls_refuse_to_be_traced():
     from diffsvc_amd import muon
