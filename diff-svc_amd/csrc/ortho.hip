@@ -306,9 +306,9 @@ __device__ __forceinline__ void transpose_tile(const half4 (&v)[4], const half8 
 }
 
 // One workgroup = a tile of (32 TM WR) x (32 TN WC) of one matrix (or one K slice of it): WR x WC waves, a wave = TM x TN accumulator tiles; NST stages
-// of KS k steps in LDS.  Bound by the matrix cores where the tiles are large: X <- M X of [4096, 4096] bf16 124 us (1108 TFLOP/s; the same library product
-// runs at 1214), of [20, 768, 1152] fp32 109 us (27 GFLOP in three MFMAs each: 749 TFLOP/s of fp16).  A tile of 64 reads two fragments per MFMA from LDS, which
-// halves that (X X^T of [2048, 8192] bf16 64 us, 541 TFLOP/s), and one [384, 384] product is 6.6 us of latency.
+// of KS k steps in LDS.  Bound by the matrix cores where the tiles are large: X <- M X of [4096, 4096] 350 us (137 GFLOP in three MFMAs each: 1178 TFLOP/s
+// of fp16; the library's bf16 product runs at 1214), on one plane 124 us (1108), of [20, 768, 1152] 106 us (768).  A tile of 64 reads two fragments per MFMA from
+// LDS (X X^T of [2048, 8192] 136 us, 780 TFLOP/s, on one plane 64 us, 541), and one [384, 384] product is 6.9 us of latency.
 template <int P_, int TM_, int TN_, int WR_, int WC_, int KS_, int NST_, int PER_CU_>
 struct Tile {
     static constexpr int P = P_, TM = TM_, TN = TN_, WR = WR_, WC = WC_, KS = KS_, NST = NST_, PER_CU = PER_CU_;
@@ -791,8 +791,8 @@ struct Cut {
     int kind, size, tiles_i, n_tiles, full, rest, slices;
     long long part_bytes() const { return slices > 1 ? (long long)rest * slices * size * size * 4 : 0; }
 };
-// A slice keeps at least 16 stages: a partial tile's way through memory costs about as much as 8 ([4, 1024, 1024] bf16: 253 us whole, 344 us in slices of
-// 8 or more; [100, 4000] fp32: 250 us whole, 124 us in slices of 16; the last 16 of [4096, 4096] bf16's 528 tiles: 1783 -> 1638 us).
+// A slice keeps at least 16 stages: a partial tile's way through memory costs about as much as 8 ([4, 1024, 1024] on one plane: 253 us whole, 344 us in
+// slices of 8 or more; [100, 4000] fp32: 250 us whole, 124 us in slices of 16; the last 16 of [4096, 4096]'s 528 tiles on one plane: 1783 -> 1638 us).
 constexpr int MIN_STAGES = 16;
 template <class C>
 Cut cut_for(int kind, bool sym, int batch, int mi, int nj, int k16) {
@@ -817,7 +817,7 @@ template <int P>
 Cut cut(bool sym, int batch, int mi, int nj, int k16) {
     // 128 where that gives about every CU a tile ([1000, 3000] fp32 on 36 ... 192 tiles of 128 by four waves: 665 us, on tiles of 64: 376 us; [2048, 2048]'s
     // symmetric products on 136 tiles in K slices: 869 us, on tiles of 64: 781 us).  256 where it still gives one to each and nothing is padded for it
-    // ([4096, 4096] bf16, the full product: 158 -> 140 us)
+    // ([4096, 4096] on one plane, the full product: 158 -> 140 us)
     const int t = mi / 128;
     const long long tiles = (long long)batch * (sym ? t * (t + 1) / 2 : (long long)t * (nj / 128));
     if (P == 1 && !sym && mi % 256 == 0 && nj % 256 == 0 && tiles >= 4 * CUS) return cut_for<typename Tiles<1, 256>::type>(256, sym, batch, mi, nj, k16);

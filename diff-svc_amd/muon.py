@@ -3,7 +3,7 @@
   X = G / (||G||_F + eps);  steps times:  A = X X^T,  X <- (a I + b A + c A A) X;  O = scale * X
 
 takes every singular value s of the normalised update through s (a + b s^2 + c s^4): with the default coefficients all of them end between about
-0.7 and 1.2, so O is close to U V^T of G = U S V^T.  ``muon_step_`` orthogonalises the (Nesterov) momentum of a gradient and takes the weight step.
+0.7 and 1.2, so O is close to U V^T of G = U S V^T.  (Coefficients under which the iterate shrinks lose the bits that it shrinks by.)  ``muon_step_`` orthogonalises the (Nesterov) momentum of a gradient and takes the weight step.
 
 Types: float32, float16 and bfloat16 tensors run on split fp16 operands (``precision="f16_x3"``, the default: fp32-class, three matrix-core products
 per product).  ``"f16"`` asks for single fp16 operands: up to three times as fast, but a rounding of an early iterate grows by up to a^steps where the

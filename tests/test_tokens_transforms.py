@@ -107,6 +107,25 @@ def test_func_transforms(dev):
         assert torch.equal(f.vmap(ours, (0, None))(tb, w), plain(tb, w))
 
 
+@pytest.mark.gpu
+def test_func_transforms_of_the_module():
+    """With the module's flag in the call; what torch's older batching cannot look into is refused, not answered."""
+    m = T.TokenEmbeddingHip(V, H, padding_idx=PAD, scale=SCALE).cuda()
+    m.weight.data.copy_(small(V, H, dev="cuda"))
+    t, wb = tokens("cuda", 3, 6, seed=7), small(3, V, H, seed=8, dev="cuda")
+    assert torch.equal(torch.func.vmap(m)(t), plain(t, m.weight))
+    call = lambda w, t: torch.func.functional_call(m, {"weight": w}, (t,))
+    assert torch.equal(torch.func.vmap(call)(wb, t), torch.stack([plain(a, b) for a, b in zip(t, wb)]))
+    assert torch.equal(torch.func.grad(lambda w: (call(w, t) ** 2).sum())(wb[0]), torch.func.grad(lambda w: (plain(t, w) ** 2).sum())(wb[0]))
+    m.check()
+    t[1, 2] = V
+    torch.func.vmap(m)(t)
+    with pytest.raises(IndexError):
+        m.check()
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(m(t[0]), m.weight, small(4, 6, H, seed=2, dev="cuda"), is_grads_batched=True)
+
+
 @pytest.mark.parametrize("trained", [False, True])
 def test_trace(dev, trained, tmp_path):
     """A traced lookup is the lookup, on tokens, tables and shapes that it was not traced on, with its gradient and its flag, saved and loaded too."""
